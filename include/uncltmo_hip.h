@@ -714,6 +714,127 @@ size_t uncl_optical_flow_workspace_bytes(int H, int W);
 int uncl_optical_flow(const float* img_to_align, const float* img_source, int H, int W, float* flow, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------
+ * Operators on rows of channels.  A row is one pixel or graph node of a channel-last tensor: `cols` consecutive elements, rows `ld*`
+ * elements apart (ld >= cols, any alignment of the element type).  Elements are fp32, bf16 or fp16 (`dtype`); sums, statistics and
+ * weight gradients are fp32.  The reference composes its bottleneck of DropPath, residual additions and 1x1 convolutions
+ * (Unet_singleFrame.py:25-41, torch_vertex.py:181-227); these are the forms a wider bottleneck needs beside uncl_scale_rows,
+ * uncl_inorm_act / uncl_bnorm_act and uncl_conv_igemm.  Calls with no elements return UNCL_OK and launch nothing.
+ * ---------------------------------------------------------------------------------------------------- */
+/* 8-bit floating-point formats (OCP) */
+#define UNCL_Q8_NONE 0
+#define UNCL_E4M3 1 /* largest number 448   */
+#define UNCL_E5M2 2 /* largest number 57344 */
+
+/* y = res + keep * x * 65536 / (65536 - t), t = round(p * 65536): the probability is held in 16 bits (p < 2^-17 drops nothing), and the
+ * factor is that of the rounded one.  keep of (row, c) = [word >= t], word = the (c % 8)-th 16-bit half (low half first) of
+ * Philox4x32-10 (Salmon et al., SC 2011) with key = seed (low, high) and counter = ((row / span) * ceil(cols / 8) + c / 8 (low, high),
+ * offset (low, high)).  span = 1: every element has its own flag; span = H * W of an NHWC tensor: whole channels of a sample are dropped
+ * (nn.Dropout2d).  seed_dev (device memory, 2 x uint64 {seed, offset}; NULL: the host's `seed`) is read by every launch, so that a
+ * captured graph draws new flags when its program changes it between replays; the host's `offset` is added to it.  The mask is never
+ * stored: the gradient of x is the same call on the gradient of y.  Dropped elements are 0 even where x is infinite or NaN.  p = 1 drops
+ * everything.  res may be NULL; y may be x or res. */
+int uncl_dropout(const void* x, long long ldx, const void* res, long long ldr, void* y, long long ldy, int dtype, long long rows,
+                 int cols, float p, long long span, const unsigned long long* seed_dev, unsigned long long seed,
+                 unsigned long long offset, void* stream);
+
+/* h = round(res + drop(x)) (the sum is normalised as stored), r = 1 / sqrt(mean over the row of h^2 + eps), y = h * r * weight.
+ * res, weight (fp32 [cols]), h, rstd (fp32 [rows], what the backward pass needs) may be NULL; p = 0: nothing is dropped, else
+ * p / span / seed_dev / seed / offset as in uncl_dropout.  h may be x or res.  y_fmt != UNCL_Q8_NONE: y is written in that 8-bit format with
+ * one scale for each 128 channels of a row (see uncl_quant8), y_scale[row * scale_row + block * scale_block]; ldy in bytes then. */
+typedef struct uncl_rmsnorm_desc {
+  int dtype, y_fmt;
+  long long rows;
+  int cols;
+  float eps; /* > 0 */
+  const void* x;
+  long long ldx;
+  const void* res;
+  long long ldr;
+  const float* weight;
+  void* h;
+  long long ldh;
+  void* y;
+  long long ldy;
+  float* rstd;
+  float* y_scale;
+  long long scale_row, scale_block;
+  float p;
+  long long span; /* >= 1 */
+  const unsigned long long* seed_dev;
+  unsigned long long seed, offset;
+} uncl_rmsnorm_desc;
+int uncl_rmsnorm(const uncl_rmsnorm_desc* d, void* stream);
+
+/* Its gradients, with n = h * rstd:  g = gh + rstd * (gy * weight - n * mean(gy * weight * n));  g_res = g, g_x = drop(g) with the forward
+ * call's flags, g_w = sum over the rows of gy * n (fixed order: the same inputs give the same bits).  gy, gh (the gradient that flows
+ * into h beside y's) and each output may be NULL; outputs may be the inputs gy / gh of the same place.  workspace:
+ * uncl_rmsnorm_backward_workspace_bytes(rows, cols), needed with g_w only. */
+typedef struct uncl_rmsnorm_bwd_desc {
+  int dtype;
+  int cols;
+  long long rows;
+  const void* gy;
+  long long ldgy;
+  const void* gh;
+  long long ldgh;
+  const void* h;
+  long long ldh;
+  const float* weight;
+  const float* rstd;
+  void* g_res;
+  long long ldgr;
+  void* g_x;
+  long long ldgx;
+  float* g_w;
+  float p;
+  long long span;
+  const unsigned long long* seed_dev;
+  unsigned long long seed, offset;
+} uncl_rmsnorm_bwd_desc;
+size_t uncl_rmsnorm_backward_workspace_bytes(long long rows, int cols);
+int uncl_rmsnorm_backward(const uncl_rmsnorm_bwd_desc* d, void* workspace, void* stream);
+
+/* out[c] = sum over the rows of x (fp32, fixed order; zeros for no rows): the bias gradient of a linear layer, any width and type
+ * (uncl_colsum_bf16: the generator's own layers) */
+size_t uncl_row_sum_workspace_bytes(long long rows, int cols);
+int uncl_row_sum(const void* x, int dtype, long long rows, int cols, long long ld, float* out, void* workspace, void* stream);
+
+/* 8-bit operands with one fp32 scale for each block: scale = max(amax, 2^-100) * fl(1 / largest), q = round-to-nearest-even of
+ * x * fl(1 / scale).  amax is over the finite elements of the block; an infinity becomes the largest number, a NaN stays NaN.
+ * tile = 0: blocks of 128 along the rows of q (1 x 128); tile = 1: blocks of 128 x 128.  transposed = 1: q is x's transpose (cols rows of
+ * `rows` elements, blocks of 128 along x's rows).  q: bytes, rows ldq bytes apart (bytes behind a row's end are not written);
+ * scale[r * scale_row + b * scale_block], r = row of q (tile: row / 128), b = block along it. */
+int uncl_quant8(const void* x, int dtype, long long rows, int cols, long long ldx, void* q, long long ldq, int fmt, float* scale,
+                long long scale_row, long long scale_block, int tile, int transposed, void* stream);
+
+/* out[m][n] = act(sum over k of a[m][k] sa[m][k / 128] * b[n][k] sb[..][k / 128] + bias[n]) + res[m][n], a (M, K) and b (N, K) in 8 bits,
+ * any M, N, K; rows start on 16-byte borders (pointers and lda / ldb multiples of 16 bytes) and are readable up to the next multiple of
+ * 16 bytes behind K (what stands there has no effect).  a_scale[m * a_scale_row + kb * a_scale_block]; b_scale likewise by n (b_tile = 0) or
+ * n / 128 (b_tile = 1).  bias fp32 [N] or NULL; act UNCL_ACT_*; res (type of out) or NULL, may be out.  Sums are fp32, in an order that
+ * depends on the sizes and types alone.  With a bf16 result and over 64 rows, products are added up by the 8-bit matrix instruction, which
+ * cuts each off 13 bits under the largest power of two among its eight neighbours along k: about 1e-4 of the result, a tenth of its
+ * rounding.  fp16 and fp32 results do without that. */
+typedef struct uncl_matmul8_desc {
+  int M, N, K;
+  int a_fmt, b_fmt, b_tile;
+  const void* a;
+  long long lda;
+  const float* a_scale;
+  long long a_scale_row, a_scale_block;
+  const void* b;
+  long long ldb;
+  const float* b_scale;
+  long long b_scale_row, b_scale_block;
+  const float* bias;
+  int act, out_dtype;
+  const void* res;
+  long long ldr;
+  void* out;
+  long long ldo;
+} uncl_matmul8_desc;
+int uncl_matmul8(const uncl_matmul8_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

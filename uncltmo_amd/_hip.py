@@ -16,6 +16,7 @@ F32, BF16, F16 = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_LRELU, ACT_GELU, ACT_SIGMOID, ACT_TANH, ACT_MSIG = 0, 1, 2, 3, 4, 5, 6
 SRC_PLAIN, SRC_MAXPOOL2, SRC_CONCAT_SSR, SRC_CONCAT2, SRC_IMAGE1, SRC_CONCAT_SSR_UP = 0, 1, 2, 3, 4, 5
 Z_NONE, Z_GROUPS, Z_UP2X2 = 0, 1, 2
+Q8_NONE, E4M3, E5M2 = 0, 1, 2
 G_NUM_WEIGHTS = 26
 
 _ERR = {-1: "UNCL_ERR_ARG (unsupported shape / dtype / mode)", -2: "UNCL_ERR_LAUNCH", -3: "UNCL_ERR_NODEVICE"}
@@ -92,6 +93,36 @@ class UnpackItem(C.Structure):
 class PackItem(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("Cout", C.c_int), ("Cin", C.c_int), ("k", C.c_int),
                 ("transposed", C.c_int), ("flip", C.c_int), ("cout_order", C.c_int)]
+
+
+class RmsnormDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("y_fmt", C.c_int), ("rows", C.c_longlong), ("cols", C.c_int), ("eps", C.c_float),
+        ("x", C.c_void_p), ("ldx", C.c_longlong), ("res", C.c_void_p), ("ldr", C.c_longlong), ("weight", C.c_void_p),
+        ("h", C.c_void_p), ("ldh", C.c_longlong), ("y", C.c_void_p), ("ldy", C.c_longlong), ("rstd", C.c_void_p),
+        ("y_scale", C.c_void_p), ("scale_row", C.c_longlong), ("scale_block", C.c_longlong),
+        ("p", C.c_float), ("span", C.c_longlong), ("seed_dev", C.c_void_p), ("seed", C.c_ulonglong), ("offset", C.c_ulonglong),
+    ]
+
+
+class RmsnormBwdDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("cols", C.c_int), ("rows", C.c_longlong),
+        ("gy", C.c_void_p), ("ldgy", C.c_longlong), ("gh", C.c_void_p), ("ldgh", C.c_longlong), ("h", C.c_void_p), ("ldh", C.c_longlong),
+        ("weight", C.c_void_p), ("rstd", C.c_void_p), ("g_res", C.c_void_p), ("ldgr", C.c_longlong),
+        ("g_x", C.c_void_p), ("ldgx", C.c_longlong), ("g_w", C.c_void_p),
+        ("p", C.c_float), ("span", C.c_longlong), ("seed_dev", C.c_void_p), ("seed", C.c_ulonglong), ("offset", C.c_ulonglong),
+    ]
+
+
+class Matmul8Desc(C.Structure):
+    _fields_ = [
+        ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("a_fmt", C.c_int), ("b_fmt", C.c_int), ("b_tile", C.c_int),
+        ("a", C.c_void_p), ("lda", C.c_longlong), ("a_scale", C.c_void_p), ("a_scale_row", C.c_longlong), ("a_scale_block", C.c_longlong),
+        ("b", C.c_void_p), ("ldb", C.c_longlong), ("b_scale", C.c_void_p), ("b_scale_row", C.c_longlong), ("b_scale_block", C.c_longlong),
+        ("bias", C.c_void_p), ("act", C.c_int), ("out_dtype", C.c_int), ("res", C.c_void_p), ("ldr", C.c_longlong),
+        ("out", C.c_void_p), ("ldo", C.c_longlong),
+    ]
 
 
 SIGNATURES = {
@@ -258,6 +289,16 @@ SIGNATURES = {
     "uncl_tile_gather": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "uncl_tile_blend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "uncl_tile_offsets": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "uncl_dropout": (C.c_int, [C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_longlong, C.c_int,
+                               C.c_float, C.c_longlong, C.c_void_p, C.c_ulonglong, C.c_ulonglong, C.c_void_p]),
+    "uncl_rmsnorm": (C.c_int, [C.POINTER(RmsnormDesc), C.c_void_p]),
+    "uncl_rmsnorm_backward_workspace_bytes": (C.c_size_t, [C.c_longlong, C.c_int]),
+    "uncl_rmsnorm_backward": (C.c_int, [C.POINTER(RmsnormBwdDesc), C.c_void_p, C.c_void_p]),
+    "uncl_row_sum_workspace_bytes": (C.c_size_t, [C.c_longlong, C.c_int]),
+    "uncl_row_sum": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "uncl_quant8": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p,
+                              C.c_longlong, C.c_longlong, C.c_int, C.c_int, C.c_void_p]),
+    "uncl_matmul8": (C.c_int, [C.POINTER(Matmul8Desc), C.c_void_p]),
 }
 
 

@@ -1,0 +1,464 @@
+"""Operators on rows of channels: dropout from a counter, the residual addition with an RMS norm behind it, and the matrix product of 8-bit
+operands (csrc/row_ops.hip, csrc/quant8.hip, csrc/matmul8.hip).
+
+A row is one pixel or graph node: the LAST axis of a tensor holds its channels.  An (N, C, H, W) map of the generator, which lies channel-last
+in memory, goes in as `x.permute(0, 2, 3, 1)` -- a view.  Leading axes may have any strides that make one row pitch (slices of a wider
+buffer among them); other layouts are copied first.  Tensors are fp32, bf16 or fp16 on an MI355X; there is no CPU path.
+
+    training   y, h = add_rms_norm(branch, stream, weight, p=0.1, seed=seed, offset=layer)     # h: the new residual stream
+               z = linear8(y, w1, b1)                                                          # 8-bit products, forward and gradients
+    serving    q, h = rms_norm_quant8(branch, weight, residual=stream)
+               z = matmul8(q, w1_q8, bias=b1, act="gelu")                                      # w1_q8 = quantize8(w1, "tile"), once
+"""
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _hip
+
+BLOCK = 128
+_FMT = {"e4m3": _hip.E4M3, "e5m2": _hip.E5M2}
+_F8 = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
+_F8_CODE = {torch.float8_e4m3fn: _hip.E4M3, torch.float8_e5m2: _hip.E5M2}
+_ACT = {"none": _hip.ACT_NONE, "relu": _hip.ACT_RELU, "lrelu": _hip.ACT_LRELU, "gelu": _hip.ACT_GELU, "sigmoid": _hip.ACT_SIGMOID,
+        "tanh": _hip.ACT_TANH, "msig": _hip.ACT_MSIG}
+_CODE = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16, torch.float16: _hip.F16}
+_U64 = (1 << 64) - 1
+
+
+def _call(dev, what, fn, *args):
+    """One entry point of the library on the tensors' device and that device's current stream."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+    if rc:
+        _hip.check(rc, what)
+
+
+def _need(t, what, dtypes, shape=None, dev=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("uncltmo_amd: %s must be a tensor, got %s" % (what, type(t).__name__))
+    if not t.is_cuda:
+        raise _hip.HipError("%s is on %s; the HIP path needs it on the MI355X" % (what, t.device))
+    if t.dtype not in dtypes:
+        raise TypeError("uncltmo_amd: %s must be %s, got %s" % (what, " / ".join(str(d).replace("torch.", "") for d in dtypes), t.dtype))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError("uncltmo_amd: %s must have shape %s, got %s" % (what, tuple(shape), tuple(t.shape)))
+    if dev is not None and t.device != dev:
+        raise ValueError("uncltmo_amd: %s is on %s, the other tensors on %s" % (what, t.device, dev))
+    return t
+
+
+def _pitch(t):
+    """Distance between neighbouring rows in elements, or None if the rows of `t` are not evenly spaced."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        return None
+    pitch = run = None
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if pitch is None:
+            pitch, run = stride, stride * size
+        elif stride != run:
+            return None
+        else:
+            run *= size
+    pitch = t.shape[-1] if pitch is None else pitch
+    return pitch if pitch >= t.shape[-1] else None
+
+
+def _rows(t):
+    """(tensor whose rows have one pitch, pitch)"""
+    p = _pitch(t)
+    if p is None:
+        t = t.contiguous()
+        p = t.shape[-1]
+    return t, p
+
+
+def _extent(x):
+    """(rows, channels)"""
+    if x.dim() == 0:
+        raise ValueError("uncltmo_amd: a tensor of rows needs an axis of channels")
+    return x.shape[:-1].numel(), x.shape[-1]
+
+
+def _seed_args(p, seed, offset, span, dev):
+    """checked (p, span, seed tensor or None, seed, offset)"""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("uncltmo_amd: the dropout probability must be in [0, 1], got %r" % p)
+    if not isinstance(span, int) or span < 1:
+        raise ValueError("uncltmo_amd: span (rows that share their flags) must be a positive integer, got %r" % (span,))
+    if not isinstance(offset, int):
+        raise TypeError("uncltmo_amd: offset must be an integer, got %s" % type(offset).__name__)
+    if isinstance(seed, torch.Tensor):
+        _need(seed, "seed", (torch.int64,), (2,), dev)
+        if not seed.is_contiguous():
+            raise ValueError("uncltmo_amd: a seed tensor must be contiguous")
+        return p, span, seed, 0, offset & _U64
+    if not isinstance(seed, int):
+        raise TypeError("uncltmo_amd: seed must be an integer or a device tensor of two int64 (seed, offset), got %s" % type(seed).__name__)
+    return p, span, None, seed & _U64, offset & _U64
+
+
+def _dropout(x, res, drop):
+    rows, cols = _extent(x)
+    x, ldx = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    ldr = 0
+    if res is not None:
+        res, ldr = _rows(res)
+    p, span, dev_seed, seed, offset = drop
+    _call(x.device, "uncl_dropout", _hip.lib().uncl_dropout, x.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr, y.data_ptr(), cols,
+          _CODE[x.dtype], rows, cols, p, span, None if dev_seed is None else dev_seed.data_ptr(), seed, offset)
+    return y
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, res, drop):
+        ctx.drop = drop[:2] + (None,) + drop[3:]
+        ctx.on_device = drop[2] is not None
+        if ctx.on_device:
+            ctx.save_for_backward(drop[2])       # autograd refuses a backward pass whose seed was changed in between
+        return _dropout(x.detach(), None if res is None else res.detach(), drop)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        need = ctx.needs_input_grad
+        drop = ctx.drop[:2] + (ctx.saved_tensors[0],) + ctx.drop[3:] if ctx.on_device else ctx.drop
+        return _dropout(g, None, drop) if need[0] else None, g if need[1] else None, None
+
+
+def dropout(x, p, seed, offset=0, residual=None, span=1):
+    """residual + keep * x / (1 - p): the flags come from a counter (Philox4x32-10 of `seed`, `offset` and the element's place), no mask is
+    stored, and the backward pass makes the same flags again.
+
+    seed: an integer, or an int64 device tensor (seed, offset) that every launch reads -- the form for a captured graph, whose program
+    changes it in place between replays.  offset: a number of its own for each call that shares a seed (layer, step); added to the seed
+    tensor's.  span: so many consecutive rows share their flags; H * W for an (N, H, W, C) map drops whole channels of a sample, 1 single
+    elements.  p is held in 16 bits (rounded to a multiple of 2^-16, the factor with it).  Dropped elements are 0 whatever x holds.  Every
+    call drops: leave it out where nothing shall be dropped."""
+    _need(x, "x", tuple(_CODE))
+    if residual is not None:
+        _need(residual, "residual", (x.dtype,), x.shape, x.device)
+    return _DropoutFn.apply(x, residual, _seed_args(p, seed, offset, span, x.device))
+
+
+def _norm_desc(x, res, w, eps, drop):
+    d = _hip.RmsnormDesc()
+    rows, cols = _extent(x)
+    d.dtype, d.rows, d.cols, d.eps = _CODE[x.dtype], rows, cols, eps
+    x, d.ldx = _rows(x)
+    d.x = x.data_ptr()
+    if res is not None:
+        res, d.ldr = _rows(res)
+        d.res = res.data_ptr()
+    if w is not None:
+        d.weight = w.data_ptr()
+    d.span = 1
+    if drop is not None:
+        d.p, d.span, dev_seed, d.seed, d.offset = drop
+        if dev_seed is not None:
+            d.seed_dev = dev_seed.data_ptr()
+    return d, x, res
+
+
+class _NormFn(torch.autograd.Function):
+    """(x, residual, weight) -> (y, h); h is x itself where nothing is added or dropped"""
+
+    @staticmethod
+    def forward(ctx, x, res, w, eps, drop, need_grad):
+        ctx.set_materialize_grads(False)
+        xd, rd, wd = x.detach(), None if res is None else res.detach(), None if w is None else w.detach()
+        wd = None if wd is None else wd.contiguous()
+        d, xr, rr = _norm_desc(xd, rd, wd, eps, drop)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d.y, d.ldy = y.data_ptr(), d.cols
+        fresh = res is not None or drop is not None
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if fresh else xr
+        if fresh:
+            d.h, d.ldh = h.data_ptr(), d.cols
+        rstd = None
+        if need_grad:
+            rstd = torch.empty(max(1, d.rows), dtype=torch.float32, device=x.device)
+            d.rstd = rstd.data_ptr()
+        _call(x.device, "uncl_rmsnorm", _hip.lib().uncl_rmsnorm, C.byref(d))
+        ctx.drop, ctx.has = None if drop is None else drop[:2] + (None,) + drop[3:], (res is not None, w is not None, fresh)
+        if need_grad:
+            ctx.save_for_backward(h if fresh else x, rstd, w, None if drop is None else drop[2])
+        return (y, h) if fresh else (y, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gh):
+        h, rstd, w, dev_seed = ctx.saved_tensors
+        if gy is None and gh is None:
+            return (None,) * 6
+        need, dev = ctx.needs_input_grad, h.device
+        lib = _hip.lib()
+        d = _hip.RmsnormBwdDesc()
+        d.rows, d.cols = _extent(h)
+        d.dtype = _CODE[h.dtype]
+        keep = []
+        for name, t in (("gy", gy), ("gh", gh), ("h", h.detach())):
+            if t is not None:
+                t, ld = _rows(t)
+                keep.append(t)
+                setattr(d, name, t.data_ptr())
+                setattr(d, "ld" + name, ld)
+        wd = None if w is None else w.detach().contiguous()
+        d.weight, d.rstd, d.span = None if wd is None else wd.data_ptr(), rstd.data_ptr(), 1
+        drop = ctx.drop
+        g_res = g_x = g_w = ws = None
+        if need[1] or (need[0] and drop is None):
+            g_res = torch.empty(h.shape, dtype=h.dtype, device=dev)
+            d.g_res, d.ldgr = g_res.data_ptr(), d.cols
+        if drop is None:
+            g_x = g_res if need[0] else None
+        elif need[0]:
+            g_x = torch.empty(h.shape, dtype=h.dtype, device=dev)
+            d.g_x, d.ldgx = g_x.data_ptr(), d.cols
+            d.p, d.span, _, d.seed, d.offset = drop
+            if dev_seed is not None:
+                d.seed_dev = dev_seed.data_ptr()
+        if need[2]:
+            g_w = torch.empty(w.shape, dtype=torch.float32, device=dev)
+            d.g_w = g_w.data_ptr()
+            ws = torch.empty(max(1, lib.uncl_rmsnorm_backward_workspace_bytes(d.rows, d.cols)), dtype=torch.uint8, device=dev)
+        _call(dev, "uncl_rmsnorm_backward", lib.uncl_rmsnorm_backward, C.byref(d), None if ws is None else ws.data_ptr())
+        return g_x, g_res if need[1] else None, g_w, None, None, None
+
+
+def _norm_checks(x, residual, weight, eps):
+    _need(x, "x", tuple(_CODE))
+    _extent(x)
+    if residual is not None:
+        _need(residual, "residual", (x.dtype,), x.shape, x.device)
+    if weight is not None:
+        _need(weight, "weight", (torch.float32,), x.shape[-1:], x.device)
+    eps = float(eps)
+    if not eps > 0.0:
+        raise ValueError("uncltmo_amd: eps must be positive (a row of zeros has no root mean square), got %r" % eps)
+    return eps
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def rms_norm(x, weight=None, eps=1e-6):
+    """x / sqrt(mean over the channels of x^2 + eps) * weight; weight: fp32, one number a channel.  ("Pixel norm" on a channel-last map.)"""
+    eps = _norm_checks(x, None, weight, eps)
+    return _NormFn.apply(x, None, weight, eps, None, _wants_grad(x, weight))[0]
+
+
+def add_rms_norm(x, residual, weight=None, eps=1e-6, p=0.0, seed=0, offset=0, span=1):
+    """(y, h): h = residual + dropout(x, p, ...), the residual stream behind a branch, in the tensors' type, and y = rms_norm(h, weight, eps),
+    in one pass over memory.  p = 0 drops nothing; seed / offset / span as in dropout().  Gradients flow through both results."""
+    if residual is None:
+        raise TypeError("uncltmo_amd: add_rms_norm needs a residual; rms_norm is the form without one")
+    eps = _norm_checks(x, residual, weight, eps)
+    drop = _seed_args(p, seed, offset, span, x.device)
+    return _NormFn.apply(x, residual, weight, eps, drop if drop[0] > 0.0 else None, _wants_grad(x, residual, weight))
+
+
+class Quant8(NamedTuple):
+    """A matrix in 8 bits.  data: (rows, cols) float8_e4m3fn or float8_e5m2; scale: fp32, (rows, ceil(cols / 128)) for block = "row" (one for
+    128 neighbours of a row), (ceil(rows / 128), ceil(cols / 128)) for block = "tile"."""
+    data: torch.Tensor
+    scale: torch.Tensor
+    block: str
+
+    def values(self):
+        """the fp32 matrix that the 8-bit numbers and their scales stand for"""
+        r, c = self.data.shape
+        s = self.scale.repeat_interleave(BLOCK, 1)[:, :c]
+        return self.data.float() * (s if self.block == "row" else s.repeat_interleave(BLOCK, 0)[:r])
+
+
+def _fmt(fmt):
+    if fmt not in _FMT:
+        raise ValueError("uncltmo_amd: the 8-bit format must be 'e4m3' or 'e5m2', got %r" % (fmt,))
+    return _FMT[fmt]
+
+
+def _no_grad(what, *ts):
+    if _wants_grad(*ts):
+        raise RuntimeError("uncltmo_amd: %s has no gradient; call it under torch.no_grad() or on detached tensors" % what)
+
+
+def _empty8(rows, cols, fmt, block, dev):
+    """rows on 16-byte borders; row scales lie block by block, as the product reads them"""
+    pitch = -(-cols // 16) * 16
+    data = torch.empty(rows, pitch, dtype=torch.uint8, device=dev).view(_F8[fmt])[:, :cols]
+    kb = -(-cols // BLOCK)
+    scale = (torch.empty(kb, rows, dtype=torch.float32, device=dev).t() if block == "row"
+             else torch.empty(-(-rows // BLOCK), kb, dtype=torch.float32, device=dev))
+    return Quant8(data, scale, block)
+
+
+def rms_norm_quant8(x, weight=None, residual=None, eps=1e-6, fmt="e4m3"):
+    """(Quant8, h): add_rms_norm / rms_norm with y in 8 bits, one scale for 128 channels of a row, ready for matmul8; h = x + residual in
+    their type (x itself without a residual).  The rows of all leading axes, in order.  No gradient."""
+    eps = _norm_checks(x, residual, weight, eps)
+    code = _fmt(fmt)
+    _no_grad("rms_norm_quant8", x, weight, residual)
+    rows, cols = _extent(x)
+    weight = None if weight is None else weight.contiguous()
+    d, xr, rr = _norm_desc(x, residual, weight, eps, None)
+    q = _empty8(rows, cols, fmt, "row", x.device)
+    h = x
+    if residual is not None:
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d.h, d.ldh = h.data_ptr(), cols
+    d.y, d.ldy, d.y_fmt = q.data.data_ptr(), max(cols, q.data.stride(0)), code
+    d.y_scale, d.scale_row, d.scale_block = q.scale.data_ptr(), q.scale.stride(0), q.scale.stride(1)
+    _call(x.device, "uncl_rmsnorm", _hip.lib().uncl_rmsnorm, C.byref(d))
+    return q, h
+
+
+def quantize8(x, block="row", transpose=False, fmt="e4m3"):
+    """x (rows, cols) -- leading axes of a larger tensor are its rows -- in 8 bits, block by block: scale = max(amax, 2^-100) / largest number
+    of the format, data = x / scale rounded to the nearest, ties to even.  block "row": 1 x 128 (activations, gradients); "tile": 128 x 128
+    (weights).  transpose: the result is (cols, rows), its blocks along x's rows.  Infinities become the largest number, NaN stays NaN;
+    neither counts for the block's scale."""
+    _need(x, "x", tuple(_CODE))
+    code = _fmt(fmt)
+    if block not in ("row", "tile"):
+        raise ValueError("uncltmo_amd: block must be 'row' or 'tile', got %r" % (block,))
+    _no_grad("quantize8", x)
+    rows, cols = _extent(x)
+    x, ldx = _rows(x)
+    q = _empty8(cols if transpose else rows, rows if transpose else cols, fmt, block, x.device)
+    _call(x.device, "uncl_quant8", _hip.lib().uncl_quant8, x.data_ptr(), _CODE[x.dtype], rows, cols, ldx, q.data.data_ptr(), q.data.stride(0), code,
+          q.scale.data_ptr(), q.scale.stride(0), q.scale.stride(1), int(block == "tile"), int(bool(transpose)))
+    return q
+
+
+def _operand(t, what):
+    """8-bit rows as the product reads them: on 16-byte borders, readable up to the next one behind a row's end"""
+    rows, cols = t.shape
+    room = -(-cols // 16) * 16
+    end = t.storage_offset() + (rows - 1) * t.stride(0) + room
+    if (cols <= 1 or t.stride(1) == 1) and t.stride(0) >= cols and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0 and end <= t.untyped_storage().nbytes():
+        return t
+    out = torch.zeros(rows, room, dtype=torch.uint8, device=t.device)
+    out[:, :cols] = t.view(torch.uint8) if t.is_contiguous() else t.contiguous().view(torch.uint8)
+    return out.view(t.dtype)[:, :cols]
+
+
+def _quant_checks(q, what, blocks):
+    if not isinstance(q, Quant8):
+        raise TypeError("uncltmo_amd: %s must be a Quant8 (see quantize8), got %s" % (what, type(q).__name__))
+    if q.block not in blocks:
+        raise ValueError("uncltmo_amd: %s must have blocks by %s, got %r" % (what, " or ".join(blocks), q.block))
+    _need(q.data, what + ".data", tuple(_F8_CODE))
+    if q.data.dim() != 2:
+        raise ValueError("uncltmo_amd: %s.data must be a matrix, got shape %s" % (what, tuple(q.data.shape)))
+    r, c = q.data.shape
+    _need(q.scale, what + ".scale", (torch.float32,), ((r if q.block == "row" else -(-r // BLOCK)), -(-c // BLOCK)), q.data.device)
+
+
+def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16, out=None):
+    """act(a b^T + bias) + residual of 8-bit operands a (M, K; blocks by row) and b (N, K; by tile or by row): (M, N) in out_dtype, sums in fp32.
+    bias: fp32 (N); act: none / relu / lrelu / gelu / sigmoid / tanh / msig; residual: (M, N) in out_dtype.  out: a tensor of that shape and
+    type to write (the residual itself among them).  No gradient: linear8 is the form for training."""
+    _quant_checks(a, "a", ("row",))
+    _quant_checks(b, "b", ("tile", "row"))
+    dev = a.data.device
+    (m, k), (n, kb) = a.data.shape, b.data.shape
+    if k != kb or b.data.device != dev:
+        raise ValueError("uncltmo_amd: a is (M, K) = %s on %s, b (N, K) = %s on %s" % ((m, k), dev, (n, kb), b.data.device))
+    if k == 0:
+        raise ValueError("uncltmo_amd: matmul8 needs a common axis of at least one element")
+    if act not in _ACT:
+        raise ValueError("uncltmo_amd: unknown activation %r" % (act,))
+    if out_dtype not in _CODE:
+        raise TypeError("uncltmo_amd: out_dtype must be float32, bfloat16 or float16, got %s" % out_dtype)
+    d = _hip.Matmul8Desc()
+    if bias is not None:
+        bias = _need(bias, "bias", (torch.float32,), (n,), dev).contiguous()
+        d.bias = bias.data_ptr()
+    if residual is not None:
+        _need(residual, "residual", (out_dtype,), (m, n), dev)
+    _no_grad("matmul8", bias, residual, out)
+    if out is None:
+        out = torch.empty(m, n, dtype=out_dtype, device=dev)
+    else:
+        _need(out, "out", (out_dtype,), (m, n), dev)
+        if _pitch(out) is None:
+            raise ValueError("uncltmo_amd: out must have rows of neighbouring elements, got strides %s" % (out.stride(),))
+    if m == 0 or n == 0:
+        return out
+    if residual is not None:
+        residual, d.ldr = _rows(residual)
+        d.res = residual.data_ptr()
+    ad, bd = _operand(a.data, "a"), _operand(b.data, "b")
+    d.M, d.N, d.K, d.a_fmt, d.b_fmt, d.b_tile = m, n, k, _F8_CODE[ad.dtype], _F8_CODE[bd.dtype], int(b.block == "tile")
+    d.a, d.lda, d.a_scale, d.a_scale_row, d.a_scale_block = ad.data_ptr(), ad.stride(0), a.scale.data_ptr(), a.scale.stride(0), a.scale.stride(1)
+    d.b, d.ldb, d.b_scale, d.b_scale_row, d.b_scale_block = bd.data_ptr(), bd.stride(0), b.scale.data_ptr(), b.scale.stride(0), b.scale.stride(1)
+    d.act, d.out_dtype, d.out, d.ldo = _ACT[act], _CODE[out_dtype], out.data_ptr(), _pitch(out)
+    _call(dev, "uncl_matmul8", _hip.lib().uncl_matmul8, C.byref(d))
+    return out
+
+
+def _row_sum(x):
+    lib = _hip.lib()
+    rows, cols = _extent(x)
+    x, ld = _rows(x)
+    out = torch.empty(cols, dtype=torch.float32, device=x.device)
+    ws = torch.empty(max(1, lib.uncl_row_sum_workspace_bytes(rows, cols)), dtype=torch.uint8, device=x.device)
+    _call(x.device, "uncl_row_sum", lib.uncl_row_sum, x.data_ptr(), _CODE[x.dtype], rows, cols, ld, out.data_ptr(), ws.data_ptr())
+    return out
+
+
+class _Linear8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, grad_fmt):
+        xd, wd = x.detach(), w.detach()
+        ctx.save_for_backward(x, w)
+        ctx.grad_fmt, ctx.has_bias = grad_fmt, bias is not None
+        if x.shape.numel() == 0:
+            return torch.empty(*x.shape[:-1], w.shape[0], dtype=x.dtype, device=x.device)
+        y = matmul8(quantize8(xd, "row"), quantize8(wd, "tile"), bias=None if bias is None else bias.detach(), out_dtype=x.dtype)
+        return y.view(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w = (t.detach() for t in ctx.saved_tensors)
+        need, fmt = ctx.needs_input_grad, ctx.grad_fmt
+        gx = gw = gb = None
+        if x.numel() == 0:
+            return (torch.empty_like(x) if need[0] else None, torch.zeros_like(w) if need[1] else None,
+                    torch.zeros(w.shape[0], dtype=torch.float32, device=x.device) if need[2] else None, None)
+        if need[0]:
+            gx = matmul8(quantize8(g, "row", fmt=fmt), quantize8(w, "tile", transpose=True), out_dtype=x.dtype).view(x.shape)
+        if need[1]:
+            gw = matmul8(quantize8(g, "row", transpose=True, fmt=fmt), quantize8(x, "row", transpose=True), out_dtype=w.dtype)
+        if need[2]:
+            gb = _row_sum(g)
+        return gx, gw, gb, None
+
+
+def linear8(x, weight, bias=None, grad_fmt="e5m2"):
+    """x weight^T + bias with all three products of a training step in 8 bits: x and weight are quantised to e4m3 (rows / tiles of 128), the
+    gradient of the output to grad_fmt by rows -- along its columns for x's gradient, along its rows, like x, for weight's.  weight (N, K)
+    fp32, bf16 or fp16; bias fp32 (N).  The result and x's gradient have x's type, weight's gradient weight's (summed in fp32).  The rounding
+    of the operands is not differentiated (straight through)."""
+    _need(x, "x", tuple(_CODE))
+    rows, k = _extent(x)
+    _need(weight, "weight", tuple(_CODE), None, x.device)
+    if weight.dim() != 2 or weight.shape[1] != k or k == 0 or weight.shape[0] == 0:
+        raise ValueError("uncltmo_amd: weight must be (N, %d) with N > 0 and channels to sum over, got %s" % (k, tuple(weight.shape)))
+    if bias is not None:
+        _need(bias, "bias", (torch.float32,), (weight.shape[0],), x.device)
+    _fmt(grad_fmt)
+    return _Linear8Fn.apply(x, weight, bias, grad_fmt)
