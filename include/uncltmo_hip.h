@@ -795,11 +795,6 @@ typedef struct uncl_rmsnorm_bwd_desc {
 size_t uncl_rmsnorm_backward_workspace_bytes(long long rows, int cols);
 int uncl_rmsnorm_backward(const uncl_rmsnorm_bwd_desc* d, void* workspace, void* stream);
 
-/* out[c] = sum over the rows of x (fp32, fixed order; zeros for no rows): the bias gradient of a linear layer, any width and type
- * (uncl_colsum_bf16: the generator's own layers) */
-size_t uncl_row_sum_workspace_bytes(long long rows, int cols);
-int uncl_row_sum(const void* x, int dtype, long long rows, int cols, long long ld, float* out, void* workspace, void* stream);
-
 /* 8-bit operands with one fp32 scale for each block: scale = max(amax, 2^-100) * fl(1 / largest), q = round-to-nearest-even of
  * x * fl(1 / scale).  amax is over the finite elements of the block; an infinity becomes the largest number, a NaN stays NaN.
  * tile = 0: blocks of 128 along the rows of q (1 x 128); tile = 1: blocks of 128 x 128.  transposed = 1: q is x's transpose (cols rows of
@@ -808,10 +803,10 @@ int uncl_row_sum(const void* x, int dtype, long long rows, int cols, long long l
 int uncl_quant8(const void* x, int dtype, long long rows, int cols, long long ldx, void* q, long long ldq, int fmt, float* scale,
                 long long scale_row, long long scale_block, int tile, int transposed, void* stream);
 
-/* out[m][n] = act(sum over k of a[m][k] sa[m][k / 128] * b[n][k] sb[..][k / 128] + bias[n]) + res[m][n], a (M, K) and b (N, K) in 8 bits,
- * any M, N, K; rows start on 16-byte borders (pointers and lda / ldb multiples of 16 bytes) and are readable up to the next multiple of
- * 16 bytes behind K (what stands there has no effect).  a_scale[m * a_scale_row + kb * a_scale_block]; b_scale likewise by n (b_tile = 0) or
- * n / 128 (b_tile = 1).  bias fp32 [N] or NULL; act UNCL_ACT_*; res (type of out) or NULL, may be out.  Sums are fp32, in an order that
+/* out[m][n] = act(sum over k of a[m][k] sa[m][k / 128] * b[n][k] sb[..][k / 128] + bias[n]) + res[m][n], a (M, K) and b (N, K) in 8 bits
+ * (a e4m3 or e5m2, b e4m3), any M and N, K to 2^22; rows start on 16-byte borders (pointers and lda / ldb multiples of 16 bytes, at most
+ * 2^22) and are readable up to the next multiple of 16 bytes behind K (what stands there has no effect).  a_scale[m * a_scale_row + kb *
+ * a_scale_block]; b_scale likewise by n (b_tile = 0) or n / 128 (b_tile = 1); distances between rows of scales 0 to 2^20, 1 for b's with b_tile = 0.  bias fp32 [N] or NULL; act UNCL_ACT_*; res (type of out) or NULL, may be out.  Sums are fp32, in an order that
  * depends on the sizes and types alone.  With a bf16 result and over 64 rows, products are added up by the 8-bit matrix instruction, which
  * cuts each off 13 bits under the largest power of two among its eight neighbours along k: about 1e-4 of the result, a tenth of its
  * rounding.  fp16 and fp32 results do without that. */
@@ -833,7 +828,41 @@ typedef struct uncl_matmul8_desc {
   void* out;
   long long ldo;
 } uncl_matmul8_desc;
-int uncl_matmul8(const uncl_matmul8_desc* d, void* stream);
+/* scratch memory of one call (0 for most shapes): where tiles are few and K is long, workgroups share a tile's K and their fp32 sums join in a
+ * fixed order.  workspace NULL: one workgroup a tile. */
+size_t uncl_matmul8_workspace_bytes(int M, int N, int K);
+int uncl_matmul8(const uncl_matmul8_desc* d, void* workspace, void* stream);
+
+/* The linear layer of a training step from three such products: y = x w^T + bias (x (M, K), w (N, K): e4m3, rows / tiles of 128),
+ * gx = gy w (gy (M, N) in grad_fmt by rows, w by tiles), gw = gy^T x (both by 128s along M), gb = the columns' sums of gy.  x, gy, y, gx are
+ * `dtype`, w and gw `w_dtype`, bias and gb fp32.  M, N, K to 2^22.
+ * forward: for_x / for_w = which of gx / gw will be asked for; `saved` (uncl_linear8_saved_bytes) then takes w and / or x in 8 bits,
+ * transposed, which is all that the backward pass needs of them; NULL if neither.  y and bias (NULL: none) as in uncl_matmul8.
+ * backward: the same for_x / for_w and `saved`; gx, gw, gb: NULL where not wanted.  workspace: uncl_linear8_workspace_bytes(.., backward).
+ * M = 0: returns UNCL_OK and writes nothing. */
+typedef struct uncl_linear8_desc {
+  int M, N, K;
+  int dtype, w_dtype, grad_fmt;
+  int for_x, for_w;
+  const void* x;
+  long long ldx;
+  const void* w;
+  long long ldw;
+  const float* bias;
+  void* y;
+  long long ldy;
+  const void* gy;
+  long long ldgy;
+  void* gx;
+  long long ldgx;
+  void* gw;
+  long long ldgw;
+  float* gb;
+} uncl_linear8_desc;
+size_t uncl_linear8_saved_bytes(long long M, int N, int K, int for_x, int for_w);
+size_t uncl_linear8_workspace_bytes(long long M, int N, int K, int backward);
+int uncl_linear8_forward(const uncl_linear8_desc* d, void* saved, void* workspace, void* stream);
+int uncl_linear8_backward(const uncl_linear8_desc* d, const void* saved, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

@@ -294,9 +294,9 @@ def operand(rows, cols, block, fmt="e4m3", seed=0, garbage=True):
     return (data, scale, block), row_ops.Quant8(room.view(data.dtype)[:, :cols], scale.cuda(), block)
 
 
-def check_product(m, n, k, block="tile", fa="e4m3", fb="e4m3", act="none", dtype=torch.float32, bias=True, residual=False):
+def check_product(m, n, k, block="tile", fa="e4m3", act="none", dtype=torch.float32, bias=True, residual=False):
     ra, a = operand(m, k, "row", fa)
-    rb, b = operand(n, k, block, fb, seed=1)
+    rb, b = operand(n, k, block, seed=1)
     want, size = R.matmul8(ra, rb)
     bv = rnd(n, seed=3) if bias else None
     rv = rnd(m, n, dtype=dtype, seed=4) if residual else None
@@ -312,7 +312,7 @@ def check_product(m, n, k, block="tile", fa="e4m3", fb="e4m3", act="none", dtype
         want = want + rv.double()
         tol = tol + R.U * want.abs()
     out = row_ops.matmul8(a, b, bias=None if bv is None else bv.cuda(), act=act, residual=None if rv is None else rv.cuda(), out_dtype=dtype)
-    within(out, want, tol + R.HALF[dtype] * (want.abs() + tol) + (2.0 ** -25 if dtype == torch.float16 else 0.0), "product %s" % ((m, n, k, block, fa, fb, act, dtype),))
+    within(out, want, tol + R.HALF[dtype] * (want.abs() + tol) + (2.0 ** -25 if dtype == torch.float16 else 0.0), "product %s" % ((m, n, k, block, fa, act, dtype),))
     return a, b, out
 
 
@@ -324,9 +324,11 @@ def test_product_sizes(m, n, k):
 
 @pytest.mark.parametrize("m", [3, 40, 200])
 @pytest.mark.parametrize("block", ["tile", "row"])
-@pytest.mark.parametrize("fa,fb", [("e4m3", "e4m3"), ("e5m2", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e5m2")])
-def test_product_formats(m, block, fa, fb):
-    check_product(m, 200, 400, block, fa, fb)
+@pytest.mark.parametrize("fa", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_product_formats(m, block, fa, dtype):
+    check_product(m, 200, 400, block, fa, dtype=dtype)
+    check_product(m * 9, 1100, 70, block, fa, dtype=dtype)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
@@ -337,16 +339,40 @@ def test_product_outputs(dtype, m, n):
             check_product(m, n, 256, act=act, dtype=dtype, bias=residual or act != "none", residual=residual)
 
 
-@pytest.mark.parametrize("m,n,k", [(2100, 2050, 384), (28800, 256, 256), (4096, 4096, 512)])
-def test_product_of_many_tiles(m, n, k):
-    """the large shapes against fp32 products on the GPU of what the operands stand for, whose own error is as counted for ours"""
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(2100, 2050, 384), (28800, 256, 256), (4101, 3500, 1100), (300, 33000, 1024)])
+def test_product_of_many_tiles(m, n, k, dtype):
+    """the large shapes against a 64-bit product on the GPU of what the operands stand for"""
     _, a = operand(m, k, "row")
     _, b = operand(n, k, "tile", seed=1)
-    va, vb = a.values(), b.values()
-    want, size = va.double() @ vb.double().t(), va.abs() @ vb.abs().t()
-    out = row_ops.matmul8(a, b, out_dtype=torch.float32)
-    within(out, want.cpu(), ((128 + 8 + -(-k // 128)) * R.U * size.double()).cpu(), "product")
-    assert torch.equal(out, row_ops.matmul8(a, b, out_dtype=torch.float32))
+    want, size = R.matmul8(a, b)
+    out = row_ops.matmul8(a, b, out_dtype=dtype)
+    tol = (128 + 8 + -(-k // 128)) * R.U * size + (R.cut(a, b) if dtype == torch.bfloat16 else 0.0)
+    bad = (out.double() - want).abs() > tol + R.HALF[dtype] * (want.abs() + tol) + 2.0 ** -25
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist())
+    assert torch.equal(out, row_ops.matmul8(a, b, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(65, 65, 1024), (256, 200, 4608), (129, 1000, 2100), (70, 16, 30000)])
+def test_product_of_few_tiles_and_long_sums(m, n, k, dtype):
+    """workgroups share a tile's K; without scratch memory one takes all of it"""
+    check_product(m, n, k, act="gelu", dtype=dtype, residual=True)
+    a, b, out = check_product(m, n, k, "row", "e5m2", dtype=dtype)
+    assert _hip.lib().uncl_matmul8_workspace_bytes(m, n, k) > 0
+    one = torch.empty_like(out)
+    d = _hip.Matmul8Desc()
+    d.M, d.N, d.K, d.a_fmt, d.b_fmt = m, n, k, _hip.E5M2, _hip.E4M3
+    d.a, d.lda, d.a_scale, d.a_scale_row, d.a_scale_block = a.data.data_ptr(), a.data.stride(0), a.scale.data_ptr(), a.scale.stride(0), a.scale.stride(1)
+    bs = b.scale.t().contiguous()
+    d.b, d.ldb, d.b_scale, d.b_scale_row, d.b_scale_block = b.data.data_ptr(), b.data.stride(0), bs.data_ptr(), 1, n
+    bias = rnd(n, seed=3).cuda()
+    d.bias, d.out, d.ldo, d.out_dtype = bias.data_ptr(), one.data_ptr(), n, _hip.dtype_code(dtype)
+    _hip.check(_hip.lib().uncl_matmul8(d, None, _hip.stream_ptr()), "uncl_matmul8")
+    want, size = R.matmul8((a.data, a.scale, "row"), (b.data, b.scale, "row"))
+    want = (want + bias).cpu()
+    tol = (128 + 10 + -(-k // 128)) * R.U * (size.cpu() + bias.abs().double().cpu()) + (R.cut((a.data, a.scale, "row"), (b.data, b.scale, "row")).cpu() if dtype == torch.bfloat16 else 0.0)
+    within(one, want, tol + R.HALF[dtype] * (want.abs() + tol) + 2.0 ** -25, "one workgroup a tile")
 
 
 def test_product_layouts():
@@ -381,6 +407,7 @@ def test_product_refusals():
                        (lambda: row_ops.matmul8(a, b, bias=f[:7]), ValueError), (lambda: row_ops.matmul8(a, b, residual=torch.zeros(8, 8, device="cuda")), TypeError),
                        (lambda: row_ops.matmul8(a, row_ops.Quant8(b.data, b.scale[:, :0], "tile")), ValueError),
                        (lambda: row_ops.matmul8(a, row_ops.Quant8(b.data.float(), b.scale, "tile")), TypeError),
+                       (lambda: row_ops.matmul8(a, row_ops.quantize8(torch.zeros(8, 64, device="cuda"), "tile", fmt="e5m2")), TypeError),
                        (lambda: row_ops.matmul8(a, b, bias=f.requires_grad_()), RuntimeError),
                        (lambda: row_ops.matmul8(a, b, out=torch.zeros(8, 8, dtype=torch.bfloat16, device="cuda").t()[:, ::2]), ValueError),
                        (lambda: row_ops.quantize8(torch.zeros(4, 4, device="cuda"), "column"), ValueError),
@@ -433,12 +460,30 @@ def test_linear8_without_rows():
     assert y.shape == (0, 16) and gx.shape == (0, 32) and int(gw.count_nonzero()) == 0 and int(gb.count_nonzero()) == 0
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1000, 37), (20000, 8), (300, 2500)])
-def test_row_sum(rows, cols):
-    for dtype in DTYPES:
-        x = rnd(rows, cols, dtype=dtype)
-        got = row_ops._row_sum(wide(x, 3, 1))
-        within(got, x.double().sum(0), (rows // 32 + 64) * R.U * x.double().abs().sum(0))
+@pytest.mark.parametrize("which", ["x", "w", "b", "xb", "wb"])
+def test_linear8_only_the_gradients_asked_for(which):
+    x, w, b, g = rnd(200, 130, dtype=torch.bfloat16).cuda(), rnd(72, 130, seed=1).cuda(), rnd(72, seed=2).cuda(), rnd(200, 72, dtype=torch.bfloat16, seed=3).cuda()
+    full = [t.clone().requires_grad_() for t in (x, w, b)]
+    want = dict(zip("xwb", torch.autograd.grad(row_ops.linear8(*full), full, g)))
+    some = {n: t.clone().requires_grad_(n in which) for n, t in zip("xwb", (x, w, b))}
+    got = torch.autograd.grad(row_ops.linear8(some["x"], some["w"], some["b"]), [some[n] for n in which], g)
+    assert all(torch.equal(v, want[n]) for n, v in zip(which, got))
+    with torch.no_grad():
+        assert torch.equal(row_ops.linear8(*full), row_ops.linear8(x, w, b))
+
+
+def test_linear8_of_views_and_changed_operands():
+    """rows of wider buffers; x and weight changed after the forward pass: the gradients are those of the values it saw"""
+    x, w, g = rnd(150, 100, dtype=torch.bfloat16), rnd(60, 100, seed=1), rnd(150, 60, dtype=torch.bfloat16, seed=2)
+    xs, ws = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    want = torch.autograd.grad(row_ops.linear8(xs, ws), [xs, ws], g.cuda())
+    xv, wv = wide(x, 5, 3).requires_grad_(), wide(w, 3, 1).requires_grad_()
+    y = row_ops.linear8(xv, wv)
+    with torch.no_grad():
+        xv.zero_()
+        wv.zero_()
+    got = torch.autograd.grad(y, [xv, wv], wide(g, 7, 1))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
 # ---- together --------------------------------------------------------------------------------------------------------------------------

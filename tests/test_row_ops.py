@@ -36,13 +36,14 @@ def test_struct_layouts_match_the_c_side():
     exe = os.path.join(ROOT, "build", "row_ops_sizes")
     os.makedirs(os.path.dirname(exe), exist_ok=True)
     with open(exe + ".c", "w") as f:
-        f.write('#include <stdio.h>\n#include <stddef.h>\n#include "uncltmo_hip.h"\nint main(){printf("%zu %zu %zu %zu %zu %zu\\n", '
-                "sizeof(uncl_rmsnorm_desc), sizeof(uncl_rmsnorm_bwd_desc), sizeof(uncl_matmul8_desc), offsetof(uncl_rmsnorm_desc, offset), "
-                "offsetof(uncl_rmsnorm_bwd_desc, offset), offsetof(uncl_matmul8_desc, ldo));return 0;}\n")
+        f.write('#include <stdio.h>\n#include <stddef.h>\n#include "uncltmo_hip.h"\nint main(){printf("%zu %zu %zu %zu %zu %zu %zu %zu\\n", '
+                "sizeof(uncl_rmsnorm_desc), sizeof(uncl_rmsnorm_bwd_desc), sizeof(uncl_matmul8_desc), sizeof(uncl_linear8_desc), "
+                "offsetof(uncl_rmsnorm_desc, offset), offsetof(uncl_rmsnorm_bwd_desc, offset), offsetof(uncl_matmul8_desc, ldo), "
+                "offsetof(uncl_linear8_desc, gb));return 0;}\n")
     subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), exe + ".c", "-o", exe])
     got = [int(v) for v in subprocess.check_output([exe]).split()]
-    ds = (_hip.RmsnormDesc, _hip.RmsnormBwdDesc, _hip.Matmul8Desc)
-    assert got == [C.sizeof(d) for d in ds] + [ds[0].offset.offset, ds[1].offset.offset, ds[2].ldo.offset]
+    ds = (_hip.RmsnormDesc, _hip.RmsnormBwdDesc, _hip.Matmul8Desc, _hip.Linear8Desc)
+    assert got == [C.sizeof(d) for d in ds] + [ds[0].offset.offset, ds[1].offset.offset, ds[2].ldo.offset, ds[3].gb.offset]
 
 
 def test_entries_refuse_bad_arguments_before_any_launch():
@@ -81,13 +82,24 @@ def test_entries_refuse_bad_arguments_before_any_launch():
         assert quant(**kw) == bad, kw
     assert quant(rows=0, x=None) == 0
     base = dict(M=2, N=2, K=8, a_fmt=1, b_fmt=1, b_tile=1, a=p, lda=16, a_scale=p, b=p, ldb=16, b_scale=p, out=p, ldo=2, out_dtype=_hip.F32)
-    for kw in (dict(a=None), dict(b=None), dict(a_scale=None), dict(b_scale=None), dict(out=None), dict(a_fmt=0), dict(b_fmt=3), dict(lda=8), dict(lda=24), dict(ldb=20),
+    for kw in (dict(a=None), dict(b=None), dict(a_scale=None), dict(b_scale=None), dict(out=None), dict(a_fmt=0), dict(b_fmt=3), dict(b_fmt=2), dict(lda=2 ** 22 + 16), dict(a_scale_row=2 ** 20 + 1), dict(b_scale_row=-1), dict(b_tile=0, b_scale_row=2), dict(lda=8), dict(lda=24), dict(ldb=20),
                dict(K=17), dict(K=0), dict(a=p + 8), dict(b=p + 4), dict(ldo=1), dict(res=p, ldr=1), dict(act=9), dict(act=-1), dict(out_dtype=5), dict(M=-1),
                dict(M=2 ** 30 + 1), dict(M=2 ** 30, N=2 ** 30, ldo=2 ** 30)):
-        assert lib.uncl_matmul8(make(_hip.Matmul8Desc, base, **kw), None) == bad, kw
-    assert lib.uncl_matmul8(make(_hip.Matmul8Desc, base, M=0, a=None), None) == 0 and lib.uncl_matmul8(None, None) == bad
-    assert lib.uncl_row_sum(p, 5, 2, 8, 8, p, p, None) == bad and lib.uncl_row_sum(p, _hip.F32, 2, 8, 7, p, p, None) == bad
-    assert lib.uncl_row_sum(p, _hip.F32, 2, 8, 8, None, p, None) == bad and lib.uncl_row_sum(p, _hip.F32, 2, 8, 8, p, None, None) == bad
+        assert lib.uncl_matmul8(make(_hip.Matmul8Desc, base, **kw), None, None) == bad, kw
+    assert lib.uncl_matmul8(make(_hip.Matmul8Desc, base, M=0, a=None), None, None) == 0 and lib.uncl_matmul8(None, None, None) == bad
+    assert lib.uncl_matmul8_workspace_bytes(28800, 1024, 256) == 0 and lib.uncl_matmul8_workspace_bytes(256, 64, 4608) > 0 and lib.uncl_matmul8_workspace_bytes(0, 4, 4) == 0
+    base = dict(M=2, N=8, K=8, dtype=_hip.BF16, w_dtype=_hip.F32, grad_fmt=2, for_x=1, for_w=1, x=p, ldx=8, w=p, ldw=8, y=p, ldy=8, gy=p, ldgy=8, gx=p, ldgx=8, gw=p, ldgw=8)
+    both = (dict(M=-1), dict(N=0), dict(K=0), dict(M=2 ** 22 + 1), dict(N=2 ** 22 + 1), dict(dtype=3), dict(w_dtype=-1), dict(grad_fmt=0), dict(grad_fmt=3))
+    for kw in both + (dict(x=None), dict(w=None), dict(y=None), dict(ldx=7), dict(ldw=7), dict(ldy=7)):
+        assert lib.uncl_linear8_forward(make(_hip.Linear8Desc, base, **kw), p, p, None) == bad, kw
+    for kw in both + (dict(gy=None), dict(ldgy=7), dict(ldgx=7), dict(ldgw=7), dict(for_x=0), dict(for_w=0)):
+        assert lib.uncl_linear8_backward(make(_hip.Linear8Desc, base, **kw), p, p, None) == bad, kw
+    d = make(_hip.Linear8Desc, base)
+    assert lib.uncl_linear8_forward(d, None, p, None) == bad and lib.uncl_linear8_forward(d, p, None, None) == bad and lib.uncl_linear8_forward(None, p, p, None) == bad
+    assert lib.uncl_linear8_backward(d, None, p, None) == bad and lib.uncl_linear8_backward(d, p, None, None) == bad and lib.uncl_linear8_backward(None, p, p, None) == bad
+    empty = make(_hip.Linear8Desc, base, M=0, x=None)
+    assert lib.uncl_linear8_forward(empty, None, None, None) == 0 and lib.uncl_linear8_backward(empty, None, None, None) == 0
+    assert lib.uncl_linear8_saved_bytes(100, 8, 8, 0, 0) == 0 and lib.uncl_linear8_saved_bytes(0, 8, 8, 1, 1) == 0
 
 
 def test_host_tensors_and_wrong_kinds_are_refused():

@@ -115,6 +115,14 @@ class RmsnormBwdDesc(C.Structure):
     ]
 
 
+class Linear8Desc(C.Structure):
+    _fields_ = [
+        ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("dtype", C.c_int), ("w_dtype", C.c_int), ("grad_fmt", C.c_int), ("for_x", C.c_int), ("for_w", C.c_int),
+        ("x", C.c_void_p), ("ldx", C.c_longlong), ("w", C.c_void_p), ("ldw", C.c_longlong), ("bias", C.c_void_p), ("y", C.c_void_p), ("ldy", C.c_longlong),
+        ("gy", C.c_void_p), ("ldgy", C.c_longlong), ("gx", C.c_void_p), ("ldgx", C.c_longlong), ("gw", C.c_void_p), ("ldgw", C.c_longlong), ("gb", C.c_void_p),
+    ]
+
+
 class Matmul8Desc(C.Structure):
     _fields_ = [
         ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("a_fmt", C.c_int), ("b_fmt", C.c_int), ("b_tile", C.c_int),
@@ -294,11 +302,14 @@ SIGNATURES = {
     "uncl_rmsnorm": (C.c_int, [C.POINTER(RmsnormDesc), C.c_void_p]),
     "uncl_rmsnorm_backward_workspace_bytes": (C.c_size_t, [C.c_longlong, C.c_int]),
     "uncl_rmsnorm_backward": (C.c_int, [C.POINTER(RmsnormBwdDesc), C.c_void_p, C.c_void_p]),
-    "uncl_row_sum_workspace_bytes": (C.c_size_t, [C.c_longlong, C.c_int]),
-    "uncl_row_sum": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p]),
     "uncl_quant8": (C.c_int, [C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p,
                               C.c_longlong, C.c_longlong, C.c_int, C.c_int, C.c_void_p]),
-    "uncl_matmul8": (C.c_int, [C.POINTER(Matmul8Desc), C.c_void_p]),
+    "uncl_matmul8_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "uncl_matmul8": (C.c_int, [C.POINTER(Matmul8Desc), C.c_void_p, C.c_void_p]),
+    "uncl_linear8_saved_bytes": (C.c_size_t, [C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "uncl_linear8_workspace_bytes": (C.c_size_t, [C.c_longlong, C.c_int, C.c_int, C.c_int]),
+    "uncl_linear8_forward": (C.c_int, [C.POINTER(Linear8Desc), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "uncl_linear8_backward": (C.c_int, [C.POINTER(Linear8Desc), C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 
 

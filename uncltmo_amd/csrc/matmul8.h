@@ -1,0 +1,397 @@
+// Matrix product of 8-bit floating-point operands with one fp32 scale for each block of 128 along the common axis:
+//
+//   out[m][n] = act( sum_kb sa[m][kb] sb[..][kb] sum_{k in kb} a[m][k] b[n][k] + bias[n] ) + res[m][n]
+//
+// a (M, K) rows, b (N, K) rows; sa one scale a row and block, sb one a 128 x 128 tile (weights) or a row and block (gradients).  The
+// matrix instructions add up one block of 128 from zero, and the block joins the fp32 sum with one multiply-add an element: the scales
+// never touch the operands.  b is the instruction's first operand, so that a lane's four results are four neighbouring columns of one
+// row m: one scale a lane, one store of 8 or 16 bytes.  Which k a lane's 32 bytes are does not matter as long as both operands agree: a
+// lane takes the 16-byte chunks g and g + 4 of its row's 128 (g = lane / 16).
+//
+// Two ways to add up a block.  The 8-bit instruction (16x16x128) adds products eight at a time on a common exponent and cuts each of them
+// off 13 bits under the largest power of two in its group (measured, the same for all of the card's 8-bit forms; between groups it adds
+// in fp32): about 1e-4 of a result of random signs.  That is a tenth of a rounding to bf16, so results in bf16 take it.  Results in fp16
+// and fp32 would show it: there the operands are widened to bf16 in registers (exact: three or four significant bits, any exponent) and
+// go through the bf16 instruction, whose sums measured 2^-23 of the products' sizes, at half the rate.
+#pragma once
+#include "matmul8_args.h"
+#include "row_ops.h"
+
+// the tiled kernels, one file for each type of result: bf16 through the 8-bit instruction, fp16 and fp32 through the bf16 one
+int mm_tiles_bf16(const MmArgs& p, int a_fmt, bool b_tile, hipStream_t s);
+int mm_tiles_f16(const MmArgs& p, int a_fmt, bool b_tile, hipStream_t s);
+int mm_tiles_f32(const MmArgs& p, int a_fmt, bool b_tile, hipStream_t s);
+
+namespace {
+
+// a lane's 32 bytes of one row, as they are or widened to bf16
+struct Wide {
+  bf16x8 v[4];
+};
+template <int F>
+__device__ __forceinline__ Wide mm_widen(const i32x8& x) {
+  typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+  Wide w;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    bf16x2 lo, hi;
+    if constexpr (F == UNCL_E4M3) {
+      lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.f, false);
+      hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.f, true);
+    } else {
+      lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x[i], 1.f, false);
+      hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(x[i], 1.f, true);
+    }
+    w.v[i >> 1][(i & 1) * 4 + 0] = lo[0];
+    w.v[i >> 1][(i & 1) * 4 + 1] = lo[1];
+    w.v[i >> 1][(i & 1) * 4 + 2] = hi[0];
+    w.v[i >> 1][(i & 1) * 4 + 3] = hi[1];
+  }
+  return w;
+}
+template <int F, bool EXACT>
+__device__ __forceinline__ auto mm_frag(const i32x8& x) {
+  if constexpr (EXACT) return mm_widen<F>(x);
+  else return x;
+}
+// one block of 128, b's TN x 16 rows by a's 16 rows: TN results
+template <int FA, int TN>
+__device__ __forceinline__ void mm_block(const i32x8 (&b)[TN], const i32x8& a, f32x4 (&d)[TN]) {
+  const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < TN; ++j) d[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a, z, UNCL_E4M3 - 1, FA - 1, 0, 0, 0, 0);
+}
+template <int FA, int TN>
+__device__ __forceinline__ void mm_block(const Wide (&b)[TN], const Wide& a, f32x4 (&d)[TN]) {
+#pragma unroll
+  for (int j = 0; j < TN; ++j) d[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) d[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j].v[i], a.v[i], d[j], 0, 0, 0);
+}
+
+// erf by Abramowitz and Stegun 7.1.26 (off by at most 1.5e-7): the library's erff took half of a short product's time
+__device__ __forceinline__ float mm_gelu(float x) {
+  const float z = __builtin_fabsf(x) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.f));
+  float q = fmaf(t, 1.061405429f, -1.453152027f);
+  q = fmaf(t, q, 1.421413741f);
+  q = fmaf(t, q, -0.284496736f);
+  q = fmaf(t, q, 0.254829592f);
+  const float e = q * t * __builtin_amdgcn_exp2f(z * z * -1.44269504088896341f);      // 1 - erf(z)
+  return x * (x > 0.f ? 1.f - 0.5f * e : 0.5f * e);
+}
+// the rarer activations, one copy of their code
+__device__ __attribute__((noinline)) float mm_act_rare(float v, int act) { return uncl_act(v, act); }
+
+// eight neighbouring columns from n on of row m (`left` of them exist): act(v + bias) + residual, rounded once
+template <int E>
+__device__ __forceinline__ void mm_act(float* v, int act) {
+  if (act == UNCL_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = mm_gelu(v[i]);
+  } else if (act == UNCL_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = v[i] > 0.f ? v[i] : 0.f;
+  } else if (act != UNCL_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = mm_act_rare(v[i], act);
+  }
+}
+
+__device__ __forceinline__ int mm_turn(int row) { return (row >> 1) & 7; }
+
+// everything this wave has in flight has arrived, and every wave of the workgroup says so
+__device__ __forceinline__ void mm_arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// bytes from a row of a matrix on, bounds-checked by the hardware: `rows` rows `pitch` bytes apart, `len` bytes of each
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mm_buffer(const void* p, long long rows, long long pitch, long long len) {
+  const long long n = (rows - 1) * pitch + len;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)(n < 0x7fffffffll ? n : 0x7fffffffll), 0x00020000);
+}
+__device__ __forceinline__ float mm_buffer_f32(__amdgpu_buffer_rsrc_t r, int offset) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, offset, 0, 0));
+}
+
+// ---- tiles ---------------------------------------------------------------------------------------------------------------------------
+// A workgroup of WM x WN waves owns BM x BN outputs; a stage of LDS holds 128 bytes of each of its BM + BN rows, two stages.  Rows
+// come in by asynchronous 16-byte loads straight to LDS, a block ahead of the products (the scales likewise, to registers): one barrier
+// a block says both that this block has arrived and that nobody reads the stage that the next one overwrites.  Chunk c of row r lies at
+// position c ^ mm_turn(r), so that the rows that a part of a wave reads at once fall on different banks (no conflicts are counted).  The loads write LDS in
+// lane order, hence the swizzle is in the lane's global address.  Rows behind M or N are out of the buffers' bounds (their results are not
+// stored); bytes behind K, of the next row or out of bounds, are cleared in LDS.
+//
+// Workgroups go to the card's eight XCDs in turn, each with an L2 of its own: the b-th workgroup takes the (b / 8)-th tile of its XCD's
+// share, and a share runs through groups of eight rows of tiles, so that the 32 tiles at work on an XCD have few rows and columns.
+// (The second launch bound, waves a SIMD: two workgroups of 128 x 128 a CU, four or more of 64 x 64 -- and under 257 registers a wave the
+// compiler leaves the matrix instructions' results where the multiply-adds can read them.)
+template <typename T, int FA, bool BT, bool EXACT, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(const MmArgs p) {
+  constexpr int NT = WM * WN * 64, TM = BM / WM / 16, TN = BN / WN / 16, STAGE = (BM + BN) * 128;
+  constexpr int LA = BM * 8 / NT, LB = BN * 8 / NT;         // 16-byte loads a thread and stage
+  __shared__ __align__(16) unsigned char lds[2 * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
+  const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, total = tm * tn;
+  int id = blockIdx.x;
+  {
+    const int x = id & 7, share = total >> 3, more = total & 7;
+    id = x * share + (x < more ? x : more) + (id >> 3);
+  }
+  const int gr = id / (8 * tn), gm = gr * 8, rows = tm - gm < 8 ? tm - gm : 8, in = id - gr * 8 * tn;
+  const int m0 = (gm + in % rows) * BM, n0 = (in / rows) * BN;
+
+  const int lr = lane >> 3, lc0 = lane & 7, k16 = (p.K + 15) & ~15;
+  const __amdgpu_buffer_rsrc_t ra = mm_buffer(p.a + (long long)m0 * p.lda, p.M - m0, p.lda, k16);
+  const __amdgpu_buffer_rsrc_t rb = mm_buffer(p.b + (long long)n0 * p.ldb, p.N - n0, p.ldb, k16);
+  const int lc = lc0 ^ mm_turn(wave * 8 + lr);                // NT / 8 rows further on the swizzle is the same
+  const int va = (wave * 8 + lr) * (int)p.lda + lc * 16, vb = (wave * 8 + lr) * (int)p.ldb + lc * 16;
+  const int sta = (NT / 8) * (int)p.lda, stb = (NT / 8) * (int)p.ldb;
+  typedef __attribute__((address_space(3))) void* lptr;
+  auto fetch = [&](int kb) {
+    unsigned char* base = lds + (kb & 1) * STAGE + wave * 1024;
+#pragma unroll
+    for (int i = 0; i < LA; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lptr)(base + i * NT * 16), 16, va + i * sta, kb * 128, 0, 0);
+#pragma unroll
+    for (int i = 0; i < LB; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lptr)(base + BM * 128 + i * NT * 16), 16, vb + i * stb, kb * 128, 0, 0);
+  };
+
+  f32x4 acc[TN][TM];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int i = 0; i < TM; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int q = lane & 15, g = lane >> 4;
+  const int mb = m0 + wm * TM * 16, nb = n0 + wn * TN * 16;   // the wave's columns lie inside one 128-column tile of b's scales
+  const float *sap = p.sa + (long long)m0 * p.sa_row, *sbp = p.sb + (BT ? ((nb < p.N ? nb : p.N - 1) >> 7) * p.sb_row : n0);
+  const int so = (mb - m0 + q) * (int)p.sa_row * 4, sno = (nb - n0 + g * 4) * 4;
+  float sm_next[TM], sb_next = 1.f;
+  f32x4 sn_next[BT ? 1 : TN];
+  auto fetch_scales = [&](int kb) {
+    const __amdgpu_buffer_rsrc_t rs = mm_buffer(sap + kb * p.sa_blk, p.M - m0, p.sa_row * 4, 4);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) sm_next[i] = mm_buffer_f32(rs, so + i * 64 * (int)p.sa_row);
+    if constexpr (BT) {
+      sb_next = sbp[kb * p.sb_blk];
+    } else {
+      const __amdgpu_buffer_rsrc_t rn = mm_buffer(sbp + kb * p.sb_blk, p.N - n0, 4, 4);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sn_next[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rn, sno + j * 64, 0, 0));
+    }
+  };
+
+  int k0 = 0, k1 = p.KB;
+  if constexpr (BM == 64)
+    if (p.part) { k0 = blockIdx.y * p.per; k1 = k0 + p.per < p.KB ? k0 + p.per : p.KB; }
+  fetch(k0);
+  fetch_scales(k0);
+  for (int kb = k0; kb < k1; ++kb) {
+    mm_arrive();
+    float sm[TM];
+    f32x4 sn[BT ? 1 : TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) sm[i] = sm_next[i] * sb_next;
+    if constexpr (!BT)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sn[j] = sn_next[j];
+    if (kb + 1 < k1) {
+      fetch(kb + 1);
+      fetch_scales(kb + 1);
+    }
+    unsigned char* st = lds + (kb & 1) * STAGE;
+    const int have = p.K - kb * 128;
+    if (have < 128) {                                        // the last block is short: clear what lies behind K
+      for (int t = threadIdx.x; t < (BM + BN) * 8; t += NT) {
+        const int r = t >> 3, c = t & 7;
+        unsigned char* at = st + r * 128 + ((c ^ mm_turn(r)) << 4);
+        const int keep = have - c * 16;
+        if (keep <= 0) *reinterpret_cast<i32x4*>(at) = i32x4{0, 0, 0, 0};
+        else
+          for (int k = keep; k < 16; ++k) at[k] = 0;
+      }
+      mm_arrive();
+    }
+    auto frag = [&](int row) {
+      const unsigned char* r = st + row * 128;
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(r + ((g ^ mm_turn(row)) << 4));
+      const i32x4 hi = *reinterpret_cast<const i32x4*>(r + (((g + 4) ^ mm_turn(row)) << 4));
+      return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    // the products of a's rows i run while those of rows i - 1 join their sums: a matrix instruction's result is never waited for
+    decltype(mm_frag<UNCL_E4M3, EXACT>(i32x8{})) fb[TN], fa[2];
+    fa[0] = mm_frag<FA, EXACT>(frag(wm * TM * 16 + q));
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[j] = mm_frag<UNCL_E4M3, EXACT>(frag(BM + (wn * TN + j) * 16 + q));
+    f32x4 t[2][TN];
+#pragma unroll
+    for (int i = 0; i <= TM; ++i) {
+      i32x8 raw;
+      if (i + 1 < TM) raw = frag((wm * TM + i + 1) * 16 + q);
+      if (i < TM) mm_block<FA, TN>(fb, fa[i & 1], t[i & 1]);
+      if (i > 0) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][i - 1][e] = fmaf(t[(i - 1) & 1][j][e], BT ? sm[i - 1] : sm[i - 1] * sn[BT ? 0 : j][e], acc[j][i - 1][e]);
+      }
+      if (i + 1 < TM) fa[(i + 1) & 1] = mm_frag<FA, EXACT>(raw);
+      if constexpr (!EXACT) {
+        if (i == 0) {                                                             // each product as soon as its operands are read
+          __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          }
+        } else if (i < TM) {
+          if (i + 1 < TM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);      // LDS reads of the next rows
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                    // a matrix instruction,
+            __builtin_amdgcn_sched_group_barrier(0x002, BT ? 4 : 8, 0);           // the last rows' multiply-adds under it
+          }
+        }
+      } else if (i < TM) {
+        if (i + 1 < TM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+        for (int j = 0; j < 4 * TN; ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, BT ? 2 : 3, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // A lane's results are four columns of sixteen different rows: they turn round in LDS, 32 rows of the wave at a time, so that eight (or
+  // four) lanes hold one row's columns and memory sees whole lines.  Each wave has its own part of LDS, whose operations stay in order.
+  constexpr int COLS = TN * 16, PITCH = COLS + 4, LPR = COLS / 8, RPP = 64 / LPR, PASSES = 32 / RPP;
+  static_assert(WM * WN * 32 * PITCH * 4 <= 2 * STAGE && TM % 2 == 0, "the turned rows fit where the stages were");
+  mm_arrive();
+  float* w = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
+  const int r0 = lane / LPR, c0 = (lane % LPR) * 8, n = nb + c0, left = p.N - n;
+  T* out = reinterpret_cast<T*>(p.out);
+  const T* res = reinterpret_cast<const T*>(p.res);
+  if constexpr (BM == 64)
+    if (p.part) {
+      const int n8 = (p.N + 7) & ~7;
+      float* part = p.part + (long long)blockIdx.y * p.M * n8 + n;
+#pragma unroll
+      for (int ch = 0; ch < TM / 2; ++ch) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(w + (i * 16 + q) * PITCH + j * 16 + g * 4) = acc[j][ch * 2 + i];
+#pragma unroll
+        for (int t = 0; t < PASSES; ++t) {
+          const int m = mb + ch * 32 + t * RPP + r0;
+          const float* at = w + (t * RPP + r0) * PITCH + c0;
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(at), hi = *reinterpret_cast<const f32x4*>(at + 4);
+          if (m < p.M && left > 0) {
+            *reinterpret_cast<f32x4*>(part + (long long)m * n8) = lo;
+            *reinterpret_cast<f32x4*>(part + (long long)m * n8 + 4) = hi;
+          }
+        }
+      }
+      return;
+    }
+  float bias[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) bias[e] = 0.f;
+  if (p.bias && left > 0) ro_load8(p.bias + n, left, bias);
+#pragma unroll
+  for (int ch = 0; ch < TM / 2; ++ch) {
+    float r[PASSES][8];
+    if (res)
+#pragma unroll
+      for (int t = 0; t < PASSES; ++t) {
+        const int m = mb + ch * 32 + t * RPP + r0;
+        if (m < p.M && left > 0) ro_load8(res + (long long)m * p.ldr + n, left, r[t]);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(w + (i * 16 + q) * PITCH + j * 16 + g * 4) = acc[j][ch * 2 + i];
+#pragma unroll
+    for (int t = 0; t < PASSES; ++t) {
+      const int m = mb + ch * 32 + t * RPP + r0;
+      float v[8];
+      const float* at = w + (t * RPP + r0) * PITCH + c0;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(at), hi = *reinterpret_cast<const f32x4*>(at + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] = lo[e] + bias[e]; v[4 + e] = hi[e] + bias[4 + e]; }
+      mm_act<8>(v, p.act);
+      if (res)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += r[t][e];
+      if (m < p.M && left > 0) ro_store8(out + (long long)m * p.ldo + n, left, v);
+    }
+  }
+}
+
+// Time goes by rounds of workgroups over the 256 CUs.  256 x 256 tiles (8-bit instruction, b scaled by tiles) work one to a CU, a round of
+// them is four units of 256 x 128 x 128; 128 x 128 ones two to a CU, two units a round, a tenth slower a unit (8192 x 4096 x 4096: 129
+// against 146 us; 4099 x 4096 x 2048, 8 units against 6: 65 against 53 us).  64 x 64 tiles where 128 x 128 ones are at most one a CU (512 x
+// 4096 x 4096: 19 against 27 us; 2048 x 2048 x 2048 17.2 against 17.7).
+template <typename T, int FA, bool BT, bool EXACT>
+int launch_tiles(const MmArgs& p, hipStream_t s) {
+  auto tiles = [&](int t) { return (long long)((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
+  const long long t128 = tiles(128);
+  if constexpr (BT && !EXACT) {
+    if (t128 > 256 && 40 * ((tiles(256) + 255) / 256) <= 22 * ((t128 + 511) / 512)) {
+      mm_tile_kernel<T, FA, BT, EXACT, 256, 256, 2, 4><<<(unsigned)tiles(256), 512, 0, s>>>(p);
+      UNCL_CHECK_LAUNCH();
+      return UNCL_OK;
+    }
+  }
+  if (t128 > 256) mm_tile_kernel<T, FA, BT, EXACT, 128, 128, 2, 2><<<(unsigned)t128, 256, 0, s>>>(p);
+  else mm_tile_kernel<T, FA, BT, EXACT, 64, 64, 2, 2><<<dim3((unsigned)tiles(64), p.part ? (p.KB + p.per - 1) / p.per : 1), 256, 0, s>>>(p);
+  UNCL_CHECK_LAUNCH();
+  return UNCL_OK;
+}
+
+// the split tiles' partial sums, in order, with the epilogue of a whole tile
+template <typename T>
+__global__ __launch_bounds__(256) void mm_join_kernel(const MmArgs p, int splits) {
+  const int n8 = (p.N + 7) & ~7, per_row = n8 >> 3;
+  const long long total = (long long)p.M * per_row;
+  for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+    const long long m = t / per_row;
+    const int n = (int)(t - m * per_row) * 8, left = p.N - n;
+    const float* at = p.part + m * n8 + n;
+    float v[8], x[8];
+    ro_load8(at, 8, v);
+#pragma unroll 4
+    for (int s = 1; s < splits; ++s) {
+      ro_load8(at + (long long)s * p.M * n8, 8, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += x[e];
+    }
+    if (p.bias) {
+      ro_load8(p.bias + n, left, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += x[e];
+    }
+    mm_act<8>(v, p.act);
+    if (p.res) {
+      ro_load8(reinterpret_cast<const T*>(p.res) + m * p.ldr + n, left, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += x[e];
+    }
+    ro_store8(reinterpret_cast<T*>(p.out) + m * p.ldo + n, left, v);
+  }
+}
+
+template <typename T, bool EXACT>
+int launch_by_format(const MmArgs& p, int a_fmt, bool b_tile, hipStream_t s) {
+  int rc;
+  if (a_fmt == UNCL_E4M3) rc = b_tile ? launch_tiles<T, UNCL_E4M3, true, EXACT>(p, s) : launch_tiles<T, UNCL_E4M3, false, EXACT>(p, s);
+  else rc = b_tile ? launch_tiles<T, UNCL_E5M2, true, EXACT>(p, s) : launch_tiles<T, UNCL_E5M2, false, EXACT>(p, s);
+  if (rc != UNCL_OK || !p.part) return rc;
+  const long long blocks = ((long long)p.M * ((p.N + 7) >> 3) + 255) / 256;
+  mm_join_kernel<T><<<(unsigned)(blocks < 2048 ? blocks : 2048), 256, 0, s>>>(p, (p.KB + p.per - 1) / p.per);
+  UNCL_CHECK_LAUNCH();
+  return UNCL_OK;
+}
+
+}  // namespace

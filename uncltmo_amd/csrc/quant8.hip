@@ -5,6 +5,7 @@
 //
 // One pass: a block is read once, its maximum found in registers (and LDS), and written in 8 bits: bound by HBM, 2 (or 4) + 1 bytes an
 // element.
+#include "matmul8_args.h"
 #include "row_ops.h"
 
 namespace {
@@ -43,12 +44,15 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const QuantArgs a) {
   }
 }
 
-// One workgroup, one 128 x 128 tile of x, an 8 x 8 patch a thread.  TILE: one scale for the tile, else one for each output row's 128.
-// TRANS: q is (cols, rows); the bytes turn round in LDS, whose rows are 144 bytes (16-byte aligned, 36 banks apart).
-template <typename T, int FMT, bool TILE, bool TRANS>
-__global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a) {
-  __shared__ float red[TILE ? 4 : 16 * 128];
-  __shared__ __align__(16) unsigned char turn[TRANS ? 128 * 144 : 16];
+// One workgroup, one 128 x 128 tile of x, an 8 x 8 patch a thread, read once.  TILE: one scale for the tile, else one for each row's 128
+// (q) and one for each column's 128 (its transpose).  WAYS: 1 = q as x lies, 2 = transposed, 3 = both; SUMS: the columns' sums too (the bias
+// gradient of a linear layer whose output gradient this is), as partial sums [tiles of rows][cols].  The bytes of the transpose turn
+// round in LDS: rows of 132 bytes put the eight lanes that write at once eight banks apart.
+template <typename T, int FMT, bool TILE, int WAYS, bool SUMS>
+__global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a, const QuantArgs at, float* __restrict__ sums) {
+  constexpr bool COLS = (!TILE && (WAYS & 2)) || SUMS;
+  __shared__ float red[COLS ? 16 * 128 : 4];
+  __shared__ __align__(16) unsigned char turn[(WAYS & 2) ? 128 * 132 : 16];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const long long row0 = (long long)blockIdx.y * 128;
   const int col0 = blockIdx.x * 128, col = col0 + tx * 8;
@@ -60,7 +64,24 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a) {
     for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
     if (row < a.rows && col < a.cols) ro_load8(reinterpret_cast<const T*>(a.x) + row * a.ldx + col, a.cols - col, v[i]);
   }
-  float inv[8];
+  if constexpr (SUMS) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t += v[i][j];
+      red[ty * 128 + tx * 8 + j] = t;
+    }
+    __syncthreads();
+    if (threadIdx.x < 128 && col0 + (int)threadIdx.x < a.cols) {
+      float t = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) t += red[k * 128 + threadIdx.x];
+      sums[(long long)blockIdx.y * a.cols + col0 + threadIdx.x] = t;
+    }
+    __syncthreads();
+  }
+  float inv = 1.f, inv_col[8];
   if constexpr (TILE) {
     float m = 0.f;
 #pragma unroll
@@ -71,12 +92,14 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     const float s = ro_scale_of<FMT>(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float t = 1.f / s;
+    inv = 1.f / s;
+    if (threadIdx.x == 0) {
+      if (WAYS & 1) a.scale[blockIdx.y * a.ss_row + blockIdx.x * a.ss_blk] = s;
+      if (WAYS & 2) at.scale[blockIdx.x * at.ss_row + blockIdx.y * at.ss_blk] = s;
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) inv[j] = t;
-    if (threadIdx.x == 0) a.scale[TRANS ? blockIdx.x * a.ss_row + blockIdx.y * a.ss_blk : blockIdx.y * a.ss_row + blockIdx.x * a.ss_blk] = s;
-  } else {
-    static_assert(TILE || TRANS, "rows as they lie have a kernel of their own");
+    for (int j = 0; j < 8; ++j) inv_col[j] = inv;
+  } else if constexpr ((WAYS & 2) != 0) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float m = 0.f;
@@ -91,28 +114,43 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a) {
 #pragma unroll
       for (int k = 0; k < 16; ++k) m = fmaxf(m, red[k * 128 + tx * 8 + j]);
       const float s = ro_scale_of<FMT>(m);
-      inv[j] = 1.f / s;
-      if (ty == 0 && col + j < a.cols) a.scale[(long long)(col + j) * a.ss_row + blockIdx.y * a.ss_blk] = s;
+      inv_col[j] = 1.f / s;
+      if (ty == 0 && col + j < a.cols) at.scale[(long long)(col + j) * at.ss_row + blockIdx.y * at.ss_blk] = s;
     }
   }
+  if constexpr ((WAYS & 2) != 0) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+    for (int j = 0; j < 8; ++j) {
+      float f[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = ro_fit<FMT>(v[i][j], inv[j]);
-  if constexpr (!TRANS) {
+      for (int i = 0; i < 8; ++i) f[i] = ro_fit<FMT>(v[i][j], inv_col[j]);
+      unsigned* to = reinterpret_cast<unsigned*>(&turn[(tx * 8 + j) * 132 + ty * 8]);
+      to[0] = ro_pack4<FMT>(f[0], f[1], f[2], f[3]);
+      to[1] = ro_pack4<FMT>(f[4], f[5], f[6], f[7]);
+    }
+  }
+  if constexpr ((WAYS & 1) != 0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const long long row = row0 + ty * 8 + i;
-      if (row < a.rows && col < a.cols)
-        ro_store8q(a.q + row * a.ldq + col, a.cols - col, ro_pack4<FMT>(v[i][0], v[i][1], v[i][2], v[i][3]),
-                   ro_pack4<FMT>(v[i][4], v[i][5], v[i][6], v[i][7]));
-    }
-  } else {
+      if constexpr (!TILE) {
+        float m = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const u32x2 b = {ro_pack4<FMT>(v[0][j], v[1][j], v[2][j], v[3][j]), ro_pack4<FMT>(v[4][j], v[5][j], v[6][j], v[7][j])};
-      *reinterpret_cast<u32x2*>(&turn[(tx * 8 + j) * 144 + ty * 8]) = b;
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, ro_finite_abs(v[i][j]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const float s = ro_scale_of<FMT>(m);
+        inv = 1.f / s;
+        if (tx == 0 && row < a.rows) a.scale[row * a.ss_row + blockIdx.x * a.ss_blk] = s;
+      }
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = ro_fit<FMT>(v[i][j], inv);
+      if (row < a.rows && col < a.cols)
+        ro_store8q(a.q + row * a.ldq + col, a.cols - col, ro_pack4<FMT>(f[0], f[1], f[2], f[3]), ro_pack4<FMT>(f[4], f[5], f[6], f[7]));
     }
+  }
+  if constexpr ((WAYS & 2) != 0) {
     __syncthreads();
     const long long n = a.rows - (row0 + tx * 8);
     if (n > 0)
@@ -120,23 +158,26 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a) {
       for (int i = 0; i < 8; ++i) {
         const int c = ty + 16 * i;
         if (col0 + c >= a.cols) break;
-        const u32x2 b = *reinterpret_cast<const u32x2*>(&turn[c * 144 + tx * 8]);
-        ro_store8q(a.q + (long long)(col0 + c) * a.ldq + row0 + tx * 8, n < 8 ? (int)n : 8, b[0], b[1]);
+        const unsigned* from = reinterpret_cast<const unsigned*>(&turn[c * 132 + tx * 8]);
+        ro_store8q(at.q + (long long)(col0 + c) * at.ldq + row0 + tx * 8, n < 8 ? (int)n : 8, from[0], from[1]);
       }
   }
 }
 
+template <typename T, int FMT, bool TILE, int WAYS, bool SUMS = false>
+int launch_tiles(const QuantArgs& a, const QuantArgs& at, float* sums, hipStream_t s) {
+  const dim3 grid((a.cols + 127) / 128, (unsigned)((a.rows + 127) / 128));
+  quant_tile_kernel<T, FMT, TILE, WAYS, SUMS><<<grid, 256, 0, s>>>(a, at, sums);
+  UNCL_CHECK_LAUNCH();
+  return UNCL_OK;
+}
+
 template <typename T, int FMT>
 int launch_quant(const QuantArgs& a, int tile, int trans, hipStream_t s) {
-  if (!tile && !trans) {
-    const long long total = (a.rows * ((a.cols + 127) >> 7) + 15) / 16;
-    quant_rows_kernel<T, FMT><<<(int)(total < 4096 ? total : 4096), 256, 0, s>>>(a);
-  } else {
-    const dim3 grid((a.cols + 127) / 128, (unsigned)((a.rows + 127) / 128));
-    if (tile && trans) quant_tile_kernel<T, FMT, true, true><<<grid, 256, 0, s>>>(a);
-    else if (tile) quant_tile_kernel<T, FMT, true, false><<<grid, 256, 0, s>>>(a);
-    else quant_tile_kernel<T, FMT, false, true><<<grid, 256, 0, s>>>(a);
-  }
+  if (tile) return trans ? launch_tiles<T, FMT, true, 2>(a, a, nullptr, s) : launch_tiles<T, FMT, true, 1>(a, a, nullptr, s);
+  if (trans) return launch_tiles<T, FMT, false, 2>(a, a, nullptr, s);
+  const long long total = (a.rows * ((a.cols + 127) >> 7) + 15) / 16;
+  quant_rows_kernel<T, FMT><<<(int)(total < 4096 ? total : 4096), 256, 0, s>>>(a);
   UNCL_CHECK_LAUNCH();
   return UNCL_OK;
 }
@@ -156,4 +197,146 @@ extern "C" int uncl_quant8(const void* x, int dtype, long long rows, int cols, l
                      : dtype == UNCL_BF16 ? launch_quant<bf16_t, F>(a, tile, transposed, s) : launch_quant<f16_t, F>(a, tile, transposed, s))
   return fmt == UNCL_E4M3 ? BY_TYPE(UNCL_E4M3) : BY_TYPE(UNCL_E5M2);
 #undef BY_TYPE
+}
+
+// ---- the linear layer of a training step -----------------------------------------------------------------------------------------------
+// y = x w^T + b, gx = gy w, gw = gy^T x with 8-bit operands.  x and w are read once in the forward pass, for its own product (x by rows, w
+// by tiles) and, where gradients are wanted, for theirs (both transposed: a quarter to a half of the bytes that keeping x and w would
+// take); gy is read once in the backward pass for both products and the bias.
+namespace {
+
+struct LinearPlan {                      // the operands' places in one buffer, 256-byte aligned
+  size_t xq, xs, wq, ws, xt, xts, wt, wts, gq, gs, gt, gts, sums, split_y, split_gx, split_gw, end;
+};
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+long long pitch16(long long v) { return (v + 15) & ~15ll; }
+long long blocks128(long long v) { return (v + 127) >> 7; }
+
+// what the backward pass needs from the forward one: x and w transposed
+size_t plan_saved(long long M, int N, int K, bool x, bool w, LinearPlan& p) {
+  size_t at = 0;
+  auto put = [&](size_t& f, size_t bytes, bool want) { f = at; at += want ? up256(bytes) : 0; };
+  put(p.xt, (size_t)K * pitch16(M), x);
+  put(p.xts, (size_t)blocks128(M) * K * 4, x);
+  put(p.wt, (size_t)K * pitch16(N), w);
+  put(p.wts, (size_t)blocks128(K) * blocks128(N) * 4, w);
+  return at;
+}
+size_t plan_forward(long long M, int N, int K, LinearPlan& p) {
+  size_t at = 0;
+  auto put = [&](size_t& f, size_t bytes) { f = at; at += up256(bytes); };
+  put(p.xq, (size_t)M * pitch16(K));
+  put(p.xs, (size_t)blocks128(K) * M * 4);
+  put(p.wq, (size_t)N * pitch16(K));
+  put(p.ws, (size_t)blocks128(N) * blocks128(K) * 4);
+  put(p.split_y, mm_split_bytes((int)M, N, K));
+  return at;
+}
+size_t plan_backward(long long M, int N, int K, LinearPlan& p) {
+  size_t at = 0;
+  auto put = [&](size_t& f, size_t bytes) { f = at; at += up256(bytes); };
+  put(p.gq, (size_t)M * pitch16(N));
+  put(p.gs, (size_t)blocks128(N) * M * 4);
+  put(p.gt, (size_t)N * pitch16(M));
+  put(p.gts, (size_t)blocks128(M) * N * 4);
+  put(p.sums, (size_t)blocks128(M) * N * 4);
+  put(p.split_gx, mm_split_bytes((int)M, K, N));
+  put(p.split_gw, mm_split_bytes(N, K, (int)M));
+  return at;
+}
+
+bool linear_ok(const uncl_linear8_desc* d) {
+  if (!d || d->M < 0 || d->N <= 0 || d->K <= 0 || d->M > (1 << 22) || d->N > (1 << 22) || d->K > (1 << 22)) return false;      // each is a product's K
+  const bool x = d->dtype == UNCL_F32 || uncl_is_h16(d->dtype), w = d->w_dtype == UNCL_F32 || uncl_is_h16(d->w_dtype);
+  return x && w && (d->grad_fmt == UNCL_E4M3 || d->grad_fmt == UNCL_E5M2);
+}
+QuantArgs quant_args(const void* x, long long rows, int cols, long long ldx, char* q, long long ldq, char* scale, long long row, long long blk) {
+  return {x, reinterpret_cast<unsigned char*>(q), reinterpret_cast<float*>(scale), rows, ldx, ldq, row, blk, cols};
+}
+
+// x by rows and (t) by its columns' 128s; w by tiles, as it lies and (t) transposed; gy both ways and its columns' sums
+template <typename T>
+int quant_x(const QuantArgs& a, const QuantArgs& t, bool both, hipStream_t s) {
+  return both ? launch_tiles<T, UNCL_E4M3, false, 3>(a, t, nullptr, s) : launch_quant<T, UNCL_E4M3>(a, 0, 0, s);
+}
+template <typename T>
+int quant_w(const QuantArgs& a, const QuantArgs& t, bool both, hipStream_t s) {
+  return both ? launch_tiles<T, UNCL_E4M3, true, 3>(a, t, nullptr, s) : launch_tiles<T, UNCL_E4M3, true, 1>(a, t, nullptr, s);
+}
+template <typename T>
+int quant_g(const QuantArgs& a, const QuantArgs& t, int fmt, bool both, float* sums, hipStream_t s) {
+  if (!both) return fmt == UNCL_E4M3 ? launch_tiles<T, UNCL_E4M3, false, 1, true>(a, t, sums, s) : launch_tiles<T, UNCL_E5M2, false, 1, true>(a, t, sums, s);
+  return fmt == UNCL_E4M3 ? launch_tiles<T, UNCL_E4M3, false, 3, true>(a, t, sums, s) : launch_tiles<T, UNCL_E5M2, false, 3, true>(a, t, sums, s);
+}
+#define LIN_BY_TYPE(DT, F, ...) ((DT) == UNCL_F32 ? F<float>(__VA_ARGS__) : (DT) == UNCL_BF16 ? F<bf16_t>(__VA_ARGS__) : F<f16_t>(__VA_ARGS__))
+
+MmArgs product(const char* a, long long lda, const char* sa, const char* b, long long ldb, const char* sb, long long sb_row, long long sb_blk, int M, int N, int K,
+               void* out, long long ldo, int dtype) {
+  MmArgs p{};
+  p.a = reinterpret_cast<const unsigned char*>(a);
+  p.b = reinterpret_cast<const unsigned char*>(b);
+  p.sa = reinterpret_cast<const float*>(sa);
+  p.sb = reinterpret_cast<const float*>(sb);
+  p.lda = lda; p.ldb = ldb; p.sa_row = 1; p.sa_blk = M; p.sb_row = sb_row; p.sb_blk = sb_blk;
+  p.M = M; p.N = N; p.K = K; p.out = out; p.ldo = ldo; p.out_dtype = dtype;
+  return p;
+}
+
+}  // namespace
+
+extern "C" size_t uncl_linear8_saved_bytes(long long M, int N, int K, int for_x, int for_w) {
+  LinearPlan p;
+  return M > 0 && N > 0 && K > 0 ? plan_saved(M, N, K, for_w != 0, for_x != 0, p) : 0;
+}
+extern "C" size_t uncl_linear8_workspace_bytes(long long M, int N, int K, int backward) {
+  LinearPlan p;
+  return M > 0 && N > 0 && K > 0 && M <= (1 << 22) ? (backward ? plan_backward(M, N, K, p) : plan_forward(M, N, K, p)) : 0;
+}
+
+extern "C" int uncl_linear8_forward(const uncl_linear8_desc* d, void* saved, void* workspace, void* stream) {
+  if (!linear_ok(d)) return UNCL_ERR_ARG;
+  if (d->M == 0) return UNCL_OK;
+  if (!d->x || !d->w || !d->y || !workspace || d->ldx < d->K || d->ldw < d->K || d->ldy < d->N || ((d->for_x || d->for_w) && !saved)) return UNCL_ERR_ARG;
+  const int M = d->M, N = d->N, K = d->K;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  LinearPlan p{};
+  plan_saved(M, N, K, d->for_w, d->for_x, p);
+  plan_forward(M, N, K, p);
+  char *ws = reinterpret_cast<char*>(workspace), *sv = reinterpret_cast<char*>(saved);
+  const QuantArgs x = quant_args(d->x, M, K, d->ldx, ws + p.xq, pitch16(K), ws + p.xs, 1, M);
+  const QuantArgs xt = quant_args(d->x, M, K, d->ldx, sv + p.xt, pitch16(M), sv + p.xts, 1, K);
+  const QuantArgs w = quant_args(d->w, N, K, d->ldw, ws + p.wq, pitch16(K), ws + p.ws, blocks128(K), 1);
+  const QuantArgs wt = quant_args(d->w, N, K, d->ldw, sv + p.wt, pitch16(N), sv + p.wts, blocks128(N), 1);
+  int rc = LIN_BY_TYPE(d->dtype, quant_x, x, xt, d->for_w != 0, s);
+  if (rc == UNCL_OK) rc = LIN_BY_TYPE(d->w_dtype, quant_w, w, wt, d->for_x != 0, s);
+  if (rc != UNCL_OK) return rc;
+  MmArgs m = product(ws + p.xq, pitch16(K), ws + p.xs, ws + p.wq, pitch16(K), ws + p.ws, blocks128(K), 1, M, N, K, d->y, d->ldy, d->dtype);
+  m.bias = d->bias;
+  return mm_run(m, UNCL_E4M3, true, ws + p.split_y, s);
+}
+
+extern "C" int uncl_linear8_backward(const uncl_linear8_desc* d, const void* saved, void* workspace, void* stream) {
+  if (!linear_ok(d)) return UNCL_ERR_ARG;
+  if (d->M == 0) return UNCL_OK;
+  if (!d->gy || !workspace || d->ldgy < d->N || ((d->gx || d->gw) && !saved) || (d->gx && (d->ldgx < d->K || !d->for_x)) || (d->gw && (d->ldgw < d->K || !d->for_w)))
+    return UNCL_ERR_ARG;
+  const int M = d->M, N = d->N, K = d->K;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  LinearPlan p{};
+  plan_saved(M, N, K, d->for_w, d->for_x, p);
+  plan_backward(M, N, K, p);
+  char* ws = reinterpret_cast<char*>(workspace);
+  const char* sv = reinterpret_cast<const char*>(saved);
+  const QuantArgs g = quant_args(d->gy, M, N, d->ldgy, ws + p.gq, pitch16(N), ws + p.gs, 1, M);
+  const QuantArgs gt = quant_args(d->gy, M, N, d->ldgy, ws + p.gt, pitch16(M), ws + p.gts, 1, N);
+  float* sums = reinterpret_cast<float*>(ws + p.sums);
+  int rc = LIN_BY_TYPE(d->dtype, quant_g, g, gt, d->grad_fmt, d->gw != nullptr, sums, s);
+  if (rc == UNCL_OK && d->gx)
+    rc = mm_run(product(ws + p.gq, pitch16(N), ws + p.gs, sv + p.wt, pitch16(N), sv + p.wts, blocks128(N), 1, M, K, N, d->gx, d->ldgx, d->dtype), d->grad_fmt,
+                true, ws + p.split_gx, s);
+  if (rc == UNCL_OK && d->gw)
+    rc = mm_run(product(ws + p.gt, pitch16(M), ws + p.gts, sv + p.xt, pitch16(M), sv + p.xts, 1, K, N, K, M, d->gw, d->ldgw, d->w_dtype), d->grad_fmt, false,
+                ws + p.split_gw, s);
+  if (rc == UNCL_OK && d->gb) rc = ro_fold_rows(sums, (int)blocks128(M), N, d->gb, s);
+  return rc;
 }

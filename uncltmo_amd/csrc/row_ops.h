@@ -142,3 +142,6 @@ __device__ __forceinline__ void ro_store8q(unsigned char* p, int n, unsigned lo,
       if (i < n) p[i] = (unsigned char)((i < 4 ? lo : hi) >> (8 * (i & 3)));
   }
 }
+
+// out[c] = sum of `blocks` partial rows of `cols` columns, in a fixed order (row_ops.hip)
+int ro_fold_rows(const float* part, int blocks, int cols, float* out, hipStream_t s);

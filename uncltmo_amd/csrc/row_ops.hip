@@ -386,35 +386,6 @@ __global__ __launch_bounds__(256) void dropout_kernel(const DropArgs a) {
   }
 }
 
-// partial column sums of a 16-bit or fp32 matrix (the bias gradient of a linear layer): [gridDim.x][cols]
-template <typename T>
-__global__ __launch_bounds__(256) void colsum_kernel(const T* __restrict__ x, long long rows, int cols, long long ld, int lanes,
-                                                     float* __restrict__ part) {
-  __shared__ float s[256][9];
-  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, per = 256 / lanes;
-  const int col = (blockIdx.y * lanes + lane) * 8, n = cols - col;
-  float t[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = 0.f;
-  if (n > 0)
-#pragma unroll 2
-    for (long long row = (long long)blockIdx.x * per + slot; row < rows; row += (long long)gridDim.x * per) {
-      float v[8];
-      ro_load8(x + row * ld + col, n, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] += v[i];
-    }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[threadIdx.x][i] = t[i];
-  __syncthreads();
-  if (slot == 0 && n > 0) {
-    for (int k = 1; k < per; ++k)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] += s[k * lanes + lane][i];
-    ro_store8(part + (long long)blockIdx.x * cols + col, n, t);
-  }
-}
-
 int pow2_at_least(int v, int most) {
   int p = 1;
   while (p < v && p < most) p <<= 1;
@@ -504,6 +475,12 @@ bool drop_ok(float p, long long span, long long rows, int cols) {
 
 }  // namespace
 
+int ro_fold_rows(const float* part, int blocks, int cols, float* out, hipStream_t s) {
+  fold_rows_kernel<<<dim3((cols + 31) / 32), dim3(32, 32), 0, s>>>(part, blocks, cols, out);
+  UNCL_CHECK_LAUNCH();
+  return UNCL_OK;
+}
+
 extern "C" int uncl_dropout(const void* x, long long ldx, const void* res, long long ldr, void* y, long long ldy, int dtype, long long rows,
                             int cols, float p, long long span, const unsigned long long* seed_dev, unsigned long long seed,
                             unsigned long long offset, void* stream) {
@@ -553,11 +530,8 @@ extern "C" int uncl_rmsnorm_backward(const uncl_rmsnorm_bwd_desc* d, void* works
   if (!d || !dtype_ok(d->dtype) || d->rows < 0 || d->cols < 0) return UNCL_ERR_ARG;
   if (d->cols == 0) return UNCL_OK;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 fold_grid((d->cols + 31) / 32), fold_block(32, 32);
   if (d->rows == 0) {
-    if (d->g_w) fold_rows_kernel<<<fold_grid, fold_block, 0, s>>>(nullptr, 0, d->cols, d->g_w);
-    UNCL_CHECK_LAUNCH();
-    return UNCL_OK;
+    return d->g_w ? ro_fold_rows(nullptr, 0, d->cols, d->g_w, s) : UNCL_OK;
   }
   if (!d->h || !d->rstd || d->ldh < d->cols || (d->gy && d->ldgy < d->cols) || (d->gh && d->ldgh < d->cols) ||
       (d->g_res && d->ldgr < d->cols) || (d->g_x && d->ldgx < d->cols) || (d->g_w && !workspace) || !drop_ok(d->p, d->span, d->rows, d->cols))
@@ -573,34 +547,5 @@ extern "C" int uncl_rmsnorm_backward(const uncl_rmsnorm_bwd_desc* d, void* works
   const int rc = d->dtype == UNCL_F32 ? launch_norm_back<float>(a, grid, s)
                                       : d->dtype == UNCL_BF16 ? launch_norm_back<bf16_t>(a, grid, s) : launch_norm_back<f16_t>(a, grid, s);
   if (rc != UNCL_OK) return rc;
-  if (d->g_w) {
-    fold_rows_kernel<<<fold_grid, fold_block, 0, s>>>(a.part, grid, d->cols, d->g_w);
-    UNCL_CHECK_LAUNCH();
-  }
-  return UNCL_OK;
-}
-
-extern "C" size_t uncl_row_sum_workspace_bytes(long long rows, int cols) {
-  if (rows <= 0 || cols <= 0) return 0;
-  return (size_t)256 * cols * sizeof(float);
-}
-
-extern "C" int uncl_row_sum(const void* x, int dtype, long long rows, int cols, long long ld, float* out, void* workspace, void* stream) {
-  if (!dtype_ok(dtype) || rows < 0 || cols < 0) return UNCL_ERR_ARG;
-  if (cols == 0) return UNCL_OK;
-  if (!out || (rows > 0 && (!x || !workspace || ld < cols))) return UNCL_ERR_ARG;
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int groups = (cols + 7) / 8, lanes = pow2_at_least(groups, 64), per = 256 / lanes;
-  const int blocks = rows == 0 ? 0 : grid_of(rows, per * 4, 256);
-  float* part = reinterpret_cast<float*>(workspace);
-  if (blocks) {
-    const dim3 grid(blocks, (groups + lanes - 1) / lanes);
-    if (dtype == UNCL_F32) colsum_kernel<float><<<grid, 256, 0, s>>>(reinterpret_cast<const float*>(x), rows, cols, ld, lanes, part);
-    else if (dtype == UNCL_BF16) colsum_kernel<bf16_t><<<grid, 256, 0, s>>>(reinterpret_cast<const bf16_t*>(x), rows, cols, ld, lanes, part);
-    else colsum_kernel<f16_t><<<grid, 256, 0, s>>>(reinterpret_cast<const f16_t*>(x), rows, cols, ld, lanes, part);
-    UNCL_CHECK_LAUNCH();
-  }
-  fold_rows_kernel<<<dim3((cols + 31) / 32), dim3(32, 32), 0, s>>>(part, blocks, cols, out);
-  UNCL_CHECK_LAUNCH();
-  return UNCL_OK;
+  return d->g_w ? ro_fold_rows(a.part, grid, d->cols, d->g_w, s) : UNCL_OK;
 }

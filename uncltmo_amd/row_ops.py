@@ -25,16 +25,19 @@ _F8_CODE = {torch.float8_e4m3fn: _hip.E4M3, torch.float8_e5m2: _hip.E5M2}
 _ACT = {"none": _hip.ACT_NONE, "relu": _hip.ACT_RELU, "lrelu": _hip.ACT_LRELU, "gelu": _hip.ACT_GELU, "sigmoid": _hip.ACT_SIGMOID,
         "tanh": _hip.ACT_TANH, "msig": _hip.ACT_MSIG}
 _CODE = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16, torch.float16: _hip.F16}
+_DTYPES = tuple(_CODE)
 _U64 = (1 << 64) - 1
+# the handle alone of torch.cuda.current_stream(device): the Stream object around it takes 2 us of a call's 10 to make
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _call(dev, what, fn, *args):
     """One entry point of the library on the tensors' device and that device's current stream."""
     if dev.index == torch.cuda.current_device():
-        rc = fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+        rc = fn(*args, _stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+            rc = fn(*args, _stream(dev.index))
     if rc:
         _hip.check(rc, what)
 
@@ -73,6 +76,8 @@ def _pitch(t):
 
 def _rows(t):
     """(tensor whose rows have one pitch, pitch)"""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     p = _pitch(t)
     if p is None:
         t = t.contiguous()
@@ -84,7 +89,8 @@ def _extent(x):
     """(rows, channels)"""
     if x.dim() == 0:
         raise ValueError("uncltmo_amd: a tensor of rows needs an axis of channels")
-    return x.shape[:-1].numel(), x.shape[-1]
+    s = x.shape
+    return (s[0] if len(s) == 2 else s[:-1].numel()), s[-1]
 
 
 def _seed_args(p, seed, offset, span, dev):
@@ -145,10 +151,13 @@ def dropout(x, p, seed, offset=0, residual=None, span=1):
     tensor's.  span: so many consecutive rows share their flags; H * W for an (N, H, W, C) map drops whole channels of a sample, 1 single
     elements.  p is held in 16 bits (rounded to a multiple of 2^-16, the factor with it).  Dropped elements are 0 whatever x holds.  Every
     call drops: leave it out where nothing shall be dropped."""
-    _need(x, "x", tuple(_CODE))
+    _need(x, "x", _DTYPES)
     if residual is not None:
         _need(residual, "residual", (x.dtype,), x.shape, x.device)
-    return _DropoutFn.apply(x, residual, _seed_args(p, seed, offset, span, x.device))
+    drop = _seed_args(p, seed, offset, span, x.device)
+    if not _wants_grad(x, residual):
+        return _dropout(x, residual, drop)
+    return _DropoutFn.apply(x, residual, drop)
 
 
 def _norm_desc(x, res, w, eps, drop):
@@ -170,51 +179,57 @@ def _norm_desc(x, res, w, eps, drop):
     return d, x, res
 
 
+def _norm(x, res, w, eps, drop, need_grad):
+    """(y, h or None where nothing is added or dropped, 1 / rms or None, the weight as the kernel read it)"""
+    w = None if w is None else w.contiguous()
+    d, xr, rr = _norm_desc(x, res, w, eps, drop)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    d.y, d.ldy = y.data_ptr(), d.cols
+    h = rstd = None
+    if res is not None or drop is not None:
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d.h, d.ldh = h.data_ptr(), d.cols
+    if need_grad:
+        rstd = torch.empty(d.rows, dtype=torch.float32, device=x.device)
+        d.rstd = rstd.data_ptr()
+    _call(x.device, "uncl_rmsnorm", _hip.lib().uncl_rmsnorm, C.byref(d))
+    return y, h, rstd, w
+
+
 class _NormFn(torch.autograd.Function):
-    """(x, residual, weight) -> (y, h); h is x itself where nothing is added or dropped"""
+    """(x, residual, weight) -> (y, h); h is None where nothing is added or dropped"""
 
     @staticmethod
-    def forward(ctx, x, res, w, eps, drop, need_grad):
+    def forward(ctx, x, res, w, eps, drop):
         ctx.set_materialize_grads(False)
-        xd, rd, wd = x.detach(), None if res is None else res.detach(), None if w is None else w.detach()
-        wd = None if wd is None else wd.contiguous()
-        d, xr, rr = _norm_desc(xd, rd, wd, eps, drop)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        d.y, d.ldy = y.data_ptr(), d.cols
-        fresh = res is not None or drop is not None
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if fresh else xr
-        if fresh:
-            d.h, d.ldh = h.data_ptr(), d.cols
-        rstd = None
-        if need_grad:
-            rstd = torch.empty(max(1, d.rows), dtype=torch.float32, device=x.device)
-            d.rstd = rstd.data_ptr()
-        _call(x.device, "uncl_rmsnorm", _hip.lib().uncl_rmsnorm, C.byref(d))
-        ctx.drop, ctx.has = None if drop is None else drop[:2] + (None,) + drop[3:], (res is not None, w is not None, fresh)
-        if need_grad:
-            ctx.save_for_backward(h if fresh else x, rstd, w, None if drop is None else drop[2])
-        return (y, h) if fresh else (y, None)
+        y, h, rstd, wc = _norm(x, res, w, eps, drop, True)
+        ctx.drop = None if drop is None else drop[:2] + (None,) + drop[3:]
+        ctx.save_for_backward(x if h is None else h, rstd, w, None if drop is None else drop[2])
+        return y, h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy, gh):
         h, rstd, w, dev_seed = ctx.saved_tensors
         if gy is None and gh is None:
-            return (None,) * 6
+            return (None,) * 5
         need, dev = ctx.needs_input_grad, h.device
         lib = _hip.lib()
         d = _hip.RmsnormBwdDesc()
         d.rows, d.cols = _extent(h)
         d.dtype = _CODE[h.dtype]
-        keep = []
-        for name, t in (("gy", gy), ("gh", gh), ("h", h.detach())):
-            if t is not None:
-                t, ld = _rows(t)
-                keep.append(t)
-                setattr(d, name, t.data_ptr())
-                setattr(d, "ld" + name, ld)
-        wd = None if w is None else w.detach().contiguous()
-        d.weight, d.rstd, d.span = None if wd is None else wd.data_ptr(), rstd.data_ptr(), 1
+        if gy is not None:
+            gy, d.ldgy = _rows(gy)
+            d.gy = gy.data_ptr()
+        if gh is not None:
+            gh, d.ldgh = _rows(gh)
+            d.gh = gh.data_ptr()
+        h, d.ldh = _rows(h)
+        d.h = h.data_ptr()
+        if w is not None:
+            w = w.contiguous()
+            d.weight = w.data_ptr()
+        d.rstd, d.span = rstd.data_ptr(), 1
         drop = ctx.drop
         g_res = g_x = g_w = ws = None
         if need[1] or (need[0] and drop is None):
@@ -233,11 +248,11 @@ class _NormFn(torch.autograd.Function):
             d.g_w = g_w.data_ptr()
             ws = torch.empty(max(1, lib.uncl_rmsnorm_backward_workspace_bytes(d.rows, d.cols)), dtype=torch.uint8, device=dev)
         _call(dev, "uncl_rmsnorm_backward", lib.uncl_rmsnorm_backward, C.byref(d), None if ws is None else ws.data_ptr())
-        return g_x, g_res if need[1] else None, g_w, None, None, None
+        return g_x, g_res if need[1] else None, g_w, None, None
 
 
 def _norm_checks(x, residual, weight, eps):
-    _need(x, "x", tuple(_CODE))
+    _need(x, "x", _DTYPES)
     _extent(x)
     if residual is not None:
         _need(residual, "residual", (x.dtype,), x.shape, x.device)
@@ -256,7 +271,7 @@ def _wants_grad(*ts):
 def rms_norm(x, weight=None, eps=1e-6):
     """x / sqrt(mean over the channels of x^2 + eps) * weight; weight: fp32, one number a channel.  ("Pixel norm" on a channel-last map.)"""
     eps = _norm_checks(x, None, weight, eps)
-    return _NormFn.apply(x, None, weight, eps, None, _wants_grad(x, weight))[0]
+    return (_NormFn.apply(x, None, weight, eps, None) if _wants_grad(x, weight) else _norm(x, None, weight, eps, None, False))[0]
 
 
 def add_rms_norm(x, residual, weight=None, eps=1e-6, p=0.0, seed=0, offset=0, span=1):
@@ -266,7 +281,10 @@ def add_rms_norm(x, residual, weight=None, eps=1e-6, p=0.0, seed=0, offset=0, sp
         raise TypeError("uncltmo_amd: add_rms_norm needs a residual; rms_norm is the form without one")
     eps = _norm_checks(x, residual, weight, eps)
     drop = _seed_args(p, seed, offset, span, x.device)
-    return _NormFn.apply(x, residual, weight, eps, drop if drop[0] > 0.0 else None, _wants_grad(x, residual, weight))
+    drop = drop if drop[0] > 0.0 else None
+    if _wants_grad(x, residual, weight):
+        return _NormFn.apply(x, residual, weight, eps, drop)
+    return _norm(x, residual, weight, eps, drop, False)[:2]
 
 
 class Quant8(NamedTuple):
@@ -329,7 +347,7 @@ def quantize8(x, block="row", transpose=False, fmt="e4m3"):
     of the format, data = x / scale rounded to the nearest, ties to even.  block "row": 1 x 128 (activations, gradients); "tile": 128 x 128
     (weights).  transpose: the result is (cols, rows), its blocks along x's rows.  Infinities become the largest number, NaN stays NaN;
     neither counts for the block's scale."""
-    _need(x, "x", tuple(_CODE))
+    _need(x, "x", _DTYPES)
     code = _fmt(fmt)
     if block not in ("row", "tile"):
         raise ValueError("uncltmo_amd: block must be 'row' or 'tile', got %r" % (block,))
@@ -342,7 +360,7 @@ def quantize8(x, block="row", transpose=False, fmt="e4m3"):
     return q
 
 
-def _operand(t, what):
+def _operand(t):
     """8-bit rows as the product reads them: on 16-byte borders, readable up to the next one behind a row's end"""
     rows, cols = t.shape
     room = -(-cols // 16) * 16
@@ -354,12 +372,17 @@ def _operand(t, what):
     return out.view(t.dtype)[:, :cols]
 
 
-def _quant_checks(q, what, blocks):
+def _scale(t, most=1 << 20):
+    """block scales with rows as near as the product wants them: within 32-bit offsets, or neighbours"""
+    return t if (1 if most == 1 else 0) <= t.stride(0) <= most else t.t().contiguous().t()
+
+
+def _quant_checks(q, what, blocks, dtypes):
     if not isinstance(q, Quant8):
         raise TypeError("uncltmo_amd: %s must be a Quant8 (see quantize8), got %s" % (what, type(q).__name__))
     if q.block not in blocks:
         raise ValueError("uncltmo_amd: %s must have blocks by %s, got %r" % (what, " or ".join(blocks), q.block))
-    _need(q.data, what + ".data", tuple(_F8_CODE))
+    _need(q.data, what + ".data", dtypes)
     if q.data.dim() != 2:
         raise ValueError("uncltmo_amd: %s.data must be a matrix, got shape %s" % (what, tuple(q.data.shape)))
     r, c = q.data.shape
@@ -367,11 +390,12 @@ def _quant_checks(q, what, blocks):
 
 
 def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16, out=None):
-    """act(a b^T + bias) + residual of 8-bit operands a (M, K; blocks by row) and b (N, K; by tile or by row): (M, N) in out_dtype, sums in fp32.
+    """act(a b^T + bias) + residual of 8-bit operands a (M, K; e4m3 or e5m2, blocks by row) and b (N, K; e4m3, blocks by tile or by row): (M, N)
+    in out_dtype, sums in fp32.
     bias: fp32 (N); act: none / relu / lrelu / gelu / sigmoid / tanh / msig; residual: (M, N) in out_dtype.  out: a tensor of that shape and
     type to write (the residual itself among them).  No gradient: linear8 is the form for training."""
-    _quant_checks(a, "a", ("row",))
-    _quant_checks(b, "b", ("tile", "row"))
+    _quant_checks(a, "a", ("row",), tuple(_F8_CODE))
+    _quant_checks(b, "b", ("tile", "row"), (torch.float8_e4m3fn,))
     dev = a.data.device
     (m, k), (n, kb) = a.data.shape, b.data.shape
     if k != kb or b.data.device != dev:
@@ -400,51 +424,72 @@ def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16
     if residual is not None:
         residual, d.ldr = _rows(residual)
         d.res = residual.data_ptr()
-    ad, bd = _operand(a.data, "a"), _operand(b.data, "b")
+    ad, bd, sa, sb = _operand(a.data), _operand(b.data), _scale(a.scale), _scale(b.scale, 1 if b.block == "row" else 1 << 20)
     d.M, d.N, d.K, d.a_fmt, d.b_fmt, d.b_tile = m, n, k, _F8_CODE[ad.dtype], _F8_CODE[bd.dtype], int(b.block == "tile")
-    d.a, d.lda, d.a_scale, d.a_scale_row, d.a_scale_block = ad.data_ptr(), ad.stride(0), a.scale.data_ptr(), a.scale.stride(0), a.scale.stride(1)
-    d.b, d.ldb, d.b_scale, d.b_scale_row, d.b_scale_block = bd.data_ptr(), bd.stride(0), b.scale.data_ptr(), b.scale.stride(0), b.scale.stride(1)
+    d.a, d.lda, d.a_scale, d.a_scale_row, d.a_scale_block = ad.data_ptr(), ad.stride(0), sa.data_ptr(), sa.stride(0), sa.stride(1)
+    d.b, d.ldb, d.b_scale, d.b_scale_row, d.b_scale_block = bd.data_ptr(), bd.stride(0), sb.data_ptr(), sb.stride(0), sb.stride(1)
     d.act, d.out_dtype, d.out, d.ldo = _ACT[act], _CODE[out_dtype], out.data_ptr(), _pitch(out)
-    _call(dev, "uncl_matmul8", _hip.lib().uncl_matmul8, C.byref(d))
-    return out
-
-
-def _row_sum(x):
     lib = _hip.lib()
-    rows, cols = _extent(x)
-    x, ld = _rows(x)
-    out = torch.empty(cols, dtype=torch.float32, device=x.device)
-    ws = torch.empty(max(1, lib.uncl_row_sum_workspace_bytes(rows, cols)), dtype=torch.uint8, device=x.device)
-    _call(x.device, "uncl_row_sum", lib.uncl_row_sum, x.data_ptr(), _CODE[x.dtype], rows, cols, ld, out.data_ptr(), ws.data_ptr())
+    size = lib.uncl_matmul8_workspace_bytes(m, n, k) if m > 64 else 0
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _call(dev, "uncl_matmul8", lib.uncl_matmul8, C.byref(d), None if ws is None else ws.data_ptr())
     return out
+
+
+def _linear8(x, w, bias, grad_fmt, for_x, for_w):
+    """(y, what the backward pass needs: the descriptor's sizes and a buffer)"""
+    lib, dev = _hip.lib(), x.device
+    d = _hip.Linear8Desc()
+    d.M, d.K = _extent(x)
+    d.N = w.shape[0]
+    d.dtype, d.w_dtype, d.grad_fmt, d.for_x, d.for_w = _CODE[x.dtype], _CODE[w.dtype], _FMT[grad_fmt], for_x, for_w
+    y = torch.empty((*x.shape[:-1], d.N), dtype=x.dtype, device=dev)
+    if d.M == 0:
+        return y, d, None
+    x, d.ldx = _rows(x)
+    w, d.ldw = _rows(w)
+    d.x, d.w, d.y, d.ldy = x.data_ptr(), w.data_ptr(), y.data_ptr(), d.N
+    if bias is not None:
+        bias = bias.contiguous()
+        d.bias = bias.data_ptr()
+    saved = torch.empty(lib.uncl_linear8_saved_bytes(d.M, d.N, d.K, for_x, for_w), dtype=torch.uint8, device=dev) if for_x or for_w else None
+    ws = torch.empty(lib.uncl_linear8_workspace_bytes(d.M, d.N, d.K, 0), dtype=torch.uint8, device=dev)
+    _call(dev, "uncl_linear8_forward", lib.uncl_linear8_forward, C.byref(d), None if saved is None else saved.data_ptr(), ws.data_ptr())
+    return y, d, saved
 
 
 class _Linear8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, grad_fmt):
-        xd, wd = x.detach(), w.detach()
-        ctx.save_for_backward(x, w)
-        ctx.grad_fmt, ctx.has_bias = grad_fmt, bias is not None
-        if x.shape.numel() == 0:
-            return torch.empty(*x.shape[:-1], w.shape[0], dtype=x.dtype, device=x.device)
-        y = matmul8(quantize8(xd, "row"), quantize8(wd, "tile"), bias=None if bias is None else bias.detach(), out_dtype=x.dtype)
-        return y.view(*x.shape[:-1], w.shape[0])
+        need = ctx.needs_input_grad
+        y, ctx.desc, saved = _linear8(x, w, bias, grad_fmt, int(need[0]), int(need[1]))
+        ctx.save_for_backward(saved)
+        ctx.shapes = x.shape, w.dtype
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        x, w = (t.detach() for t in ctx.saved_tensors)
-        need, fmt = ctx.needs_input_grad, ctx.grad_fmt
-        gx = gw = gb = None
-        if x.numel() == 0:
-            return (torch.empty_like(x) if need[0] else None, torch.zeros_like(w) if need[1] else None,
-                    torch.zeros(w.shape[0], dtype=torch.float32, device=x.device) if need[2] else None, None)
-        if need[0]:
-            gx = matmul8(quantize8(g, "row", fmt=fmt), quantize8(w, "tile", transpose=True), out_dtype=x.dtype).view(x.shape)
-        if need[1]:
-            gw = matmul8(quantize8(g, "row", transpose=True, fmt=fmt), quantize8(x, "row", transpose=True), out_dtype=w.dtype)
-        if need[2]:
-            gb = _row_sum(g)
+        (saved,), need, lib, dev = ctx.saved_tensors, ctx.needs_input_grad, _hip.lib(), g.device
+        shape, wtype = ctx.shapes
+        f = ctx.desc
+        gx = torch.empty(shape, dtype=g.dtype, device=dev) if need[0] else None
+        gw = torch.empty(f.N, f.K, dtype=wtype, device=dev) if need[1] else None
+        gb = torch.empty(f.N, dtype=torch.float32, device=dev) if need[2] else None
+        if f.M == 0:
+            return gx, None if gw is None else gw.zero_(), None if gb is None else gb.zero_(), None
+        d = _hip.Linear8Desc()
+        d.M, d.N, d.K, d.dtype, d.w_dtype, d.grad_fmt, d.for_x, d.for_w = f.M, f.N, f.K, f.dtype, f.w_dtype, f.grad_fmt, f.for_x, f.for_w
+        g, d.ldgy = _rows(g)
+        d.gy = g.data_ptr()
+        if gx is not None:
+            d.gx, d.ldgx = gx.data_ptr(), f.K
+        if gw is not None:
+            d.gw, d.ldgw = gw.data_ptr(), f.K
+        if gb is not None:
+            d.gb = gb.data_ptr()
+        ws = torch.empty(lib.uncl_linear8_workspace_bytes(f.M, f.N, f.K, 1), dtype=torch.uint8, device=dev)
+        _call(dev, "uncl_linear8_backward", lib.uncl_linear8_backward, C.byref(d), None if saved is None else saved.data_ptr(), ws.data_ptr())
         return gx, gw, gb, None
 
 
@@ -452,13 +497,15 @@ def linear8(x, weight, bias=None, grad_fmt="e5m2"):
     """x weight^T + bias with all three products of a training step in 8 bits: x and weight are quantised to e4m3 (rows / tiles of 128), the
     gradient of the output to grad_fmt by rows -- along its columns for x's gradient, along its rows, like x, for weight's.  weight (N, K)
     fp32, bf16 or fp16; bias fp32 (N).  The result and x's gradient have x's type, weight's gradient weight's (summed in fp32).  The rounding
-    of the operands is not differentiated (straight through)."""
-    _need(x, "x", tuple(_CODE))
+    of the operands is not differentiated (straight through).  What the backward pass needs of x and weight is kept in 8 bits."""
+    _need(x, "x", _DTYPES)
     rows, k = _extent(x)
-    _need(weight, "weight", tuple(_CODE), None, x.device)
+    _need(weight, "weight", _DTYPES, None, x.device)
     if weight.dim() != 2 or weight.shape[1] != k or k == 0 or weight.shape[0] == 0:
         raise ValueError("uncltmo_amd: weight must be (N, %d) with N > 0 and channels to sum over, got %s" % (k, tuple(weight.shape)))
     if bias is not None:
         _need(bias, "bias", (torch.float32,), (weight.shape[0],), x.device)
     _fmt(grad_fmt)
+    if not _wants_grad(x, weight, bias):
+        return _linear8(x, weight, bias, grad_fmt, 0, 0)[0]
     return _Linear8Fn.apply(x, weight, bias, grad_fmt)
