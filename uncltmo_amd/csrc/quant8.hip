@@ -27,19 +27,17 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const QuantArgs a) {
     const long long i = i0 + (threadIdx.x >> 4);
     const long long row = i / blocks;
     const int kb = (int)(i - row * blocks), col = kb * 128 + lane * 8, n = i < total ? a.cols - col : 0;
-    float v[8], m = 0.f;
+    float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
     if (n > 0) ro_load8(reinterpret_cast<const T*>(a.x) + row * a.ldx + col, n, v);
+    bool odd;
+    unsigned m = ro_size8(v, odd);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, ro_finite_abs(v[j]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    for (int o = 8; o > 0; o >>= 1) m = ro_max(m, (unsigned)__shfl_xor((int)m, o, 64));
     const float s = ro_scale_of<FMT>(m), inv = 1.f / s;
     if (n <= 0) continue;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = ro_fit<FMT>(v[j], inv);
-    ro_store8q(a.q + row * a.ldq + col, n, ro_pack4<FMT>(v[0], v[1], v[2], v[3]), ro_pack4<FMT>(v[4], v[5], v[6], v[7]));
+    ro_store8q(a.q + row * a.ldq + col, n, ro_pack8<FMT>(v, inv, odd));
     if (lane == 0) a.scale[row * a.ss_row + kb * a.ss_blk] = s;
   }
 }
@@ -48,50 +46,115 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const QuantArgs a) {
 // (q) and one for each column's 128 (its transpose).  WAYS: 1 = q as x lies, 2 = transposed, 3 = both; SUMS: the columns' sums too (the bias
 // gradient of a linear layer whose output gradient this is), as partial sums [tiles of rows][cols].  The bytes of the transpose turn
 // round in LDS: rows of 132 bytes put the eight lanes that write at once eight banks apart.
+// eight neighbours of a row as they lie in memory; their sizes (bits without the sign) compare as integers of the type's own width, two at a
+// time for the 16-bit types
+template <typename T>
+struct Bits {
+  typedef unsigned short U;
+};
+template <>
+struct Bits<float> {
+  typedef unsigned U;
+};
+template <typename T>
+struct Eight {
+  typedef typename Bits<T>::U U;
+  typedef U U8 __attribute__((ext_vector_type(8)));
+  static constexpr U sign = (U)1 << (8 * sizeof(U) - 1);
+  static constexpr U inf = sizeof(U) == 4 ? (U)RO_INF_BITS : (U)(__is_same(T, bf16_t) ? 0x7f80 : 0x7c00);
+  U8 raw;
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if (n >= 8) {
+      __builtin_memcpy(&raw, p, sizeof(raw));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) raw[j] = j < n ? __builtin_bit_cast(U, p[j]) : (U)0;
+    }
+  }
+  __device__ __forceinline__ float value(int j) const {
+    const U u = raw[j];
+    return (float)__builtin_bit_cast(T, u);
+  }
+  template <bool ODD>
+  __device__ __forceinline__ U8 sizes() const {
+    U8 s = raw & (U)(sign - 1);
+    if constexpr (ODD)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = s[j] >= inf ? (U)0 : s[j];
+    return s;
+  }
+  static __device__ __forceinline__ unsigned fp32_bits(U u) { return __builtin_bit_cast(unsigned, (float)__builtin_bit_cast(T, u)); }
+};
+
+// largest sizes of an 8 x 8 patch by row and by column
+template <typename T, bool ODD>
+__device__ __forceinline__ void patch_sizes(const Eight<T> (&v)[8], typename Eight<T>::U (&by_row)[8], typename Eight<T>::U8& by_col) {
+  typedef typename Eight<T>::U U;
+  typedef U U4 __attribute__((ext_vector_type(4)));
+  typedef U U2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const auto s = v[i].template sizes<ODD>();
+    by_col = i == 0 ? s : __builtin_elementwise_max(by_col, s);
+    const U4 t = __builtin_elementwise_max(s.lo, s.hi);
+    const U2 u = __builtin_elementwise_max(t.lo, t.hi);
+    by_row[i] = u[0] > u[1] ? u[0] : u[1];
+  }
+}
+
 template <typename T, int FMT, bool TILE, int WAYS, bool SUMS>
-__global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a, const QuantArgs at, float* __restrict__ sums) {
-  constexpr bool COLS = (!TILE && (WAYS & 2)) || SUMS;
-  __shared__ float red[COLS ? 16 * 128 : 4];
+__global__ __launch_bounds__(256, 2) void quant_tile_kernel(const QuantArgs a, const QuantArgs at, float* __restrict__ sums) {
+  __shared__ unsigned red[SUMS || (!TILE && (WAYS & 2)) ? 16 * 128 : 4];      // sizes, and sums and inverses as their bits
   __shared__ __align__(16) unsigned char turn[(WAYS & 2) ? 128 * 132 : 16];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const long long row0 = (long long)blockIdx.y * 128;
   const int col0 = blockIdx.x * 128, col = col0 + tx * 8;
-  float v[8][8];
+  Eight<T> v[8];
+  const T* from = reinterpret_cast<const T*>(a.x) + (row0 + ty * 8) * a.ldx + col;
+  if (row0 + 128 <= a.rows && col0 + 128 <= a.cols) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const long long row = row0 + ty * 8 + i;
+    for (int i = 0; i < 8; ++i) v[i].load(from + i * a.ldx, 8);
+  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    if (row < a.rows && col < a.cols) ro_load8(reinterpret_cast<const T*>(a.x) + row * a.ldx + col, a.cols - col, v[i]);
+    for (int i = 0; i < 8; ++i) v[i].load(from + i * a.ldx, row0 + ty * 8 + i < a.rows ? a.cols - col : 0);
+  }
+  typename Eight<T>::U by_row[8], all = 0;
+  typename Eight<T>::U8 by_col;
+  patch_sizes<T, false>(v, by_row, by_col);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) all = by_row[i] > all ? by_row[i] : all;
+  const bool odd = all >= Eight<T>::inf;
+  if (odd) {
+    patch_sizes<T, true>(v, by_row, by_col);
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all = by_row[i] > all ? by_row[i] : all;
   }
   if constexpr (SUMS) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float t = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t += v[i][j];
-      red[ty * 128 + tx * 8 + j] = t;
+      for (int i = 0; i < 8; ++i) t += v[i].value(j);
+      red[ty * 128 + tx * 8 + j] = __builtin_bit_cast(unsigned, t);
     }
     __syncthreads();
     if (threadIdx.x < 128 && col0 + (int)threadIdx.x < a.cols) {
       float t = 0.f;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) t += red[k * 128 + threadIdx.x];
+      for (int k = 0; k < 16; ++k) t += __builtin_bit_cast(float, red[k * 128 + threadIdx.x]);
       sums[(long long)blockIdx.y * a.cols + col0 + threadIdx.x] = t;
     }
     __syncthreads();
   }
   float inv = 1.f, inv_col[8];
   if constexpr (TILE) {
-    float m = 0.f;
+    unsigned m = Eight<T>::fp32_bits(all);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, ro_finite_abs(v[i][j]));
-    m = wave_max(m);
+    for (int o = 32; o > 0; o >>= 1) m = ro_max(m, (unsigned)__shfl_xor((int)m, o, 64));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
-    const float s = ro_scale_of<FMT>(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    const float s = ro_scale_of<FMT>(ro_max(ro_max(red[0], red[1]), ro_max(red[2], red[3])));
     inv = 1.f / s;
     if (threadIdx.x == 0) {
       if (WAYS & 1) a.scale[blockIdx.y * a.ss_row + blockIdx.x * a.ss_blk] = s;
@@ -101,32 +164,30 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a, cons
     for (int j = 0; j < 8; ++j) inv_col[j] = inv;
   } else if constexpr ((WAYS & 2) != 0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float m = 0.f;
+    for (int j = 0; j < 8; ++j) red[ty * 128 + tx * 8 + j] = Eight<T>::fp32_bits(by_col[j]);
+    __syncthreads();
+    if (threadIdx.x < 128) {                    // one thread a column: its maximum, scale and inverse
+      unsigned m = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, ro_finite_abs(v[i][j]));
-      red[ty * 128 + tx * 8 + j] = m;
+      for (int k = 0; k < 16; ++k) m = ro_max(m, red[k * 128 + threadIdx.x]);
+      const float s = ro_scale_of<FMT>(m);
+      if (col0 + (int)threadIdx.x < a.cols) at.scale[(long long)(col0 + threadIdx.x) * at.ss_row + blockIdx.y * at.ss_blk] = s;
+      red[threadIdx.x] = __builtin_bit_cast(unsigned, 1.f / s);
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float m = 0.f;
-#pragma unroll
-      for (int k = 0; k < 16; ++k) m = fmaxf(m, red[k * 128 + tx * 8 + j]);
-      const float s = ro_scale_of<FMT>(m);
-      inv_col[j] = 1.f / s;
-      if (ty == 0 && col + j < a.cols) at.scale[(long long)(col + j) * at.ss_row + blockIdx.y * at.ss_blk] = s;
-    }
+    for (int j = 0; j < 8; ++j) inv_col[j] = __builtin_bit_cast(float, red[tx * 8 + j]);
   }
   if constexpr ((WAYS & 2) != 0) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float f[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = ro_fit<FMT>(v[i][j], inv_col[j]);
+      for (int i = 0; i < 8; ++i) f[i] = v[i].value(j);
+      const u32x2 b = ro_pack8<FMT>(f, inv_col[j], odd);
       unsigned* to = reinterpret_cast<unsigned*>(&turn[(tx * 8 + j) * 132 + ty * 8]);
-      to[0] = ro_pack4<FMT>(f[0], f[1], f[2], f[3]);
-      to[1] = ro_pack4<FMT>(f[4], f[5], f[6], f[7]);
+      to[0] = b[0];
+      to[1] = b[1];
     }
   }
   if constexpr ((WAYS & 1) != 0) {
@@ -134,20 +195,17 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a, cons
     for (int i = 0; i < 8; ++i) {
       const long long row = row0 + ty * 8 + i;
       if constexpr (!TILE) {
-        float m = 0.f;
+        unsigned m = Eight<T>::fp32_bits(by_row[i]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, ro_finite_abs(v[i][j]));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        for (int o = 8; o > 0; o >>= 1) m = ro_max(m, (unsigned)__shfl_xor((int)m, o, 64));
         const float s = ro_scale_of<FMT>(m);
         inv = 1.f / s;
         if (tx == 0 && row < a.rows) a.scale[row * a.ss_row + blockIdx.x * a.ss_blk] = s;
       }
       float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = ro_fit<FMT>(v[i][j], inv);
-      if (row < a.rows && col < a.cols)
-        ro_store8q(a.q + row * a.ldq + col, a.cols - col, ro_pack4<FMT>(f[0], f[1], f[2], f[3]), ro_pack4<FMT>(f[4], f[5], f[6], f[7]));
+      for (int j = 0; j < 8; ++j) f[j] = v[i].value(j);
+      if (row < a.rows && col < a.cols) ro_store8q(a.q + row * a.ldq + col, a.cols - col, ro_pack8<FMT>(f, inv, odd));
     }
   }
   if constexpr ((WAYS & 2) != 0) {
@@ -158,8 +216,8 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(const QuantArgs a, cons
       for (int i = 0; i < 8; ++i) {
         const int c = ty + 16 * i;
         if (col0 + c >= a.cols) break;
-        const unsigned* from = reinterpret_cast<const unsigned*>(&turn[c * 132 + tx * 8]);
-        ro_store8q(at.q + (long long)(col0 + c) * at.ldq + row0 + tx * 8, n < 8 ? (int)n : 8, from[0], from[1]);
+        const unsigned* b = reinterpret_cast<const unsigned*>(&turn[c * 132 + tx * 8]);
+        ro_store8q(at.q + (long long)(col0 + c) * at.ldq + row0 + tx * 8, n < 8 ? (int)n : 8, u32x2{b[0], b[1]});
       }
   }
 }

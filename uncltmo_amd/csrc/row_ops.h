@@ -104,19 +104,41 @@ template <int FMT>
 struct RoF8 {
   static constexpr float top = FMT == UNCL_E4M3 ? 448.f : 57344.f;
 };
-__device__ __forceinline__ float ro_finite_abs(float v) {
-  const float a = __builtin_fabsf(v);
-  return a <= 3.402823466e38f ? a : 0.f;
+// Sizes are compared as integers (|x| without its sign orders like its bits; no canonicalising of inputs, three to an instruction): an
+// infinity or a NaN is then the largest, and only a thread that meets one (ODD) pays for leaving it out and for the clamp below.
+#define RO_INF_BITS 0x7f800000u
+template <bool ODD>
+__device__ __forceinline__ unsigned ro_size(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v) & 0x7fffffffu;
+  return ODD && u >= RO_INF_BITS ? 0u : u;
+}
+__device__ __forceinline__ unsigned ro_max(unsigned a, unsigned b) { return a > b ? a : b; }
+// largest finite size of eight; odd: whether one of them is not finite
+__device__ __forceinline__ unsigned ro_size8(const float* v, bool& odd) {
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = ro_max(m, ro_size<false>(v[i]));
+  odd = m >= RO_INF_BITS;
+  if (odd) {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = ro_max(m, ro_size<true>(v[i]));
+  }
+  return m;
 }
 template <int FMT>
-__device__ __forceinline__ float ro_scale_of(float amax) {
+__device__ __forceinline__ float ro_scale_of(unsigned amax_bits) {
 #pragma clang fp contract(off)
-  return fmaxf(amax, RO_AMAX_MIN) * (1.0f / RoF8<FMT>::top);
+  return fmaxf(__builtin_bit_cast(float, amax_bits), RO_AMAX_MIN) * (1.0f / RoF8<FMT>::top);
 }
-template <int FMT>
+// x / scale kept inside +-top, ready to be rounded (the quotient of a block's largest may be one fp32 step over top, which the conversion
+// would make a NaN)
+template <int FMT, bool ODD>
 __device__ __forceinline__ float ro_fit(float v, float inv) {
 #pragma clang fp contract(off)
-  const float q = v * inv, c = fminf(fmaxf(q, -RoF8<FMT>::top), RoF8<FMT>::top);
+  const float q = v * inv;
+  if (!ODD) return __builtin_amdgcn_fmed3f(q, -RoF8<FMT>::top, RoF8<FMT>::top);
+  const float c = fminf(fmaxf(q, -RoF8<FMT>::top), RoF8<FMT>::top);
   return q != q ? q : c;
 }
 template <int FMT>
@@ -131,15 +153,26 @@ __device__ __forceinline__ unsigned ro_pack4(float a, float b, float c, float d)
   }
   return (unsigned)v;
 }
+template <int FMT>
+__device__ __forceinline__ u32x2 ro_pack8(const float* v, float inv, bool odd) {
+  float f[8];
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = ro_fit<FMT, true>(v[i], inv);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = ro_fit<FMT, false>(v[i], inv);
+  }
+  return u32x2{ro_pack4<FMT>(f[0], f[1], f[2], f[3]), ro_pack4<FMT>(f[4], f[5], f[6], f[7])};
+}
 // eight 8-bit values to a row whose next n bytes exist
-__device__ __forceinline__ void ro_store8q(unsigned char* p, int n, unsigned lo, unsigned hi) {
+__device__ __forceinline__ void ro_store8q(unsigned char* p, int n, u32x2 v) {
   if (n >= 8) {
-    const u32x2 v = {lo, hi};
     __builtin_memcpy(p, &v, 8);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = (unsigned char)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+      if (i < n) p[i] = (unsigned char)(v[i >> 2] >> (8 * (i & 3)));
   }
 }
 

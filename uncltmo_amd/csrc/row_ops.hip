@@ -98,17 +98,13 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a) {
       if constexpr (FMT == UNCL_Q8_NONE) {
         if (n > 0) ro_store8(reinterpret_cast<T*>(a.y) + row * a.ldy + col, n, y);
       } else {
-        float m = 0.f;
+        bool odd;
+        unsigned m = ro_size8(y, odd);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, i < n ? ro_finite_abs(y[i]) : 0.f);
-#pragma unroll
-        for (int o = (LANES < 16 ? LANES : 16) / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        for (int o = (LANES < 16 ? LANES : 16) / 2; o > 0; o >>= 1) m = ro_max(m, (unsigned)__shfl_xor((int)m, o, 64));
         const float s = ro_scale_of<FMT>(m), inv = 1.f / s;
         if (n > 0) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = ro_fit<FMT>(y[i], inv);
-          ro_store8q(reinterpret_cast<unsigned char*>(a.y) + row * a.ldy + col, n, ro_pack4<FMT>(y[0], y[1], y[2], y[3]),
-                     ro_pack4<FMT>(y[4], y[5], y[6], y[7]));
+          ro_store8q(reinterpret_cast<unsigned char*>(a.y) + row * a.ldy + col, n, ro_pack8<FMT>(y, inv, odd));
           if ((col & 127) == 0) a.scale[row * a.ss_row + (col >> 7) * a.ss_blk] = s;
         }
       }
@@ -163,17 +159,13 @@ __global__ __launch_bounds__(256) void norm_long_kernel(const NormArgs a) {
       if constexpr (FMT == UNCL_Q8_NONE) {
         if (n > 0) ro_store8(reinterpret_cast<T*>(a.y) + row * a.ldy + col, n, v);
       } else {
-        float m = 0.f;
+        bool odd;
+        unsigned m = ro_size8(v, odd);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, i < n ? ro_finite_abs(v[i]) : 0.f);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        for (int o = 8; o > 0; o >>= 1) m = ro_max(m, (unsigned)__shfl_xor((int)m, o, 64));
         const float s = ro_scale_of<FMT>(m), inv = 1.f / s;
         if (n > 0) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = ro_fit<FMT>(v[i], inv);
-          ro_store8q(reinterpret_cast<unsigned char*>(a.y) + row * a.ldy + col, n, ro_pack4<FMT>(v[0], v[1], v[2], v[3]),
-                     ro_pack4<FMT>(v[4], v[5], v[6], v[7]));
+          ro_store8q(reinterpret_cast<unsigned char*>(a.y) + row * a.ldy + col, n, ro_pack8<FMT>(v, inv, odd));
           if ((col & 127) == 0) a.scale[row * a.ss_row + (col >> 7) * a.ss_blk] = s;
         }
       }

@@ -21,6 +21,7 @@ from . import _hip
 BLOCK = 128
 _FMT = {"e4m3": _hip.E4M3, "e5m2": _hip.E5M2}
 _F8 = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
+_F8_TYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
 _F8_CODE = {torch.float8_e4m3fn: _hip.E4M3, torch.float8_e5m2: _hip.E5M2}
 _ACT = {"none": _hip.ACT_NONE, "relu": _hip.ACT_RELU, "lrelu": _hip.ACT_LRELU, "gelu": _hip.ACT_GELU, "sigmoid": _hip.ACT_SIGMOID,
         "tanh": _hip.ACT_TANH, "msig": _hip.ACT_MSIG}
@@ -43,6 +44,8 @@ def _call(dev, what, fn, *args):
 
 
 def _need(t, what, dtypes, shape=None, dev=None):
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and (shape is None or t.shape == shape) and (dev is None or t.device == dev):
+        return t
     if not isinstance(t, torch.Tensor):
         raise TypeError("uncltmo_amd: %s must be a tensor, got %s" % (what, type(t).__name__))
     if not t.is_cuda:
@@ -51,9 +54,7 @@ def _need(t, what, dtypes, shape=None, dev=None):
         raise TypeError("uncltmo_amd: %s must be %s, got %s" % (what, " / ".join(str(d).replace("torch.", "") for d in dtypes), t.dtype))
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError("uncltmo_amd: %s must have shape %s, got %s" % (what, tuple(shape), tuple(t.shape)))
-    if dev is not None and t.device != dev:
-        raise ValueError("uncltmo_amd: %s is on %s, the other tensors on %s" % (what, t.device, dev))
-    return t
+    raise ValueError("uncltmo_amd: %s is on %s, the other tensors on %s" % (what, t.device, dev))
 
 
 def _pitch(t):
@@ -180,7 +181,7 @@ def _norm_desc(x, res, w, eps, drop):
 
 
 def _norm(x, res, w, eps, drop, need_grad):
-    """(y, h or None where nothing is added or dropped, 1 / rms or None, the weight as the kernel read it)"""
+    """(y, h or None where nothing is added or dropped, 1 / rms or None)"""
     w = None if w is None else w.contiguous()
     d, xr, rr = _norm_desc(x, res, w, eps, drop)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -193,7 +194,7 @@ def _norm(x, res, w, eps, drop, need_grad):
         rstd = torch.empty(d.rows, dtype=torch.float32, device=x.device)
         d.rstd = rstd.data_ptr()
     _call(x.device, "uncl_rmsnorm", _hip.lib().uncl_rmsnorm, C.byref(d))
-    return y, h, rstd, w
+    return y, h, rstd
 
 
 class _NormFn(torch.autograd.Function):
@@ -202,9 +203,15 @@ class _NormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, res, w, eps, drop):
         ctx.set_materialize_grads(False)
-        y, h, rstd, wc = _norm(x, res, w, eps, drop, True)
-        ctx.drop = None if drop is None else drop[:2] + (None,) + drop[3:]
+        y, h, rstd = _norm(x, res, w, eps, drop, True)
         ctx.save_for_backward(x if h is None else h, rstd, w, None if drop is None else drop[2])
+        # the backward pass runs on autograd's own thread, where Python is slow: what is known now is filled in now
+        d = ctx.desc = _hip.RmsnormBwdDesc()
+        d.rows, d.cols = _extent(x)
+        d.dtype, d.span = _CODE[x.dtype], 1
+        ctx.drop = drop is not None
+        if drop is not None:
+            d.p, d.span, _, d.seed, d.offset = drop
         return y, h
 
     @staticmethod
@@ -213,11 +220,8 @@ class _NormFn(torch.autograd.Function):
         h, rstd, w, dev_seed = ctx.saved_tensors
         if gy is None and gh is None:
             return (None,) * 5
-        need, dev = ctx.needs_input_grad, h.device
-        lib = _hip.lib()
-        d = _hip.RmsnormBwdDesc()
-        d.rows, d.cols = _extent(h)
-        d.dtype = _CODE[h.dtype]
+        need, dev, d, lib = ctx.needs_input_grad, h.device, _hip.RmsnormBwdDesc(), _hip.lib()
+        C.memmove(C.byref(d), C.byref(ctx.desc), C.sizeof(d))
         if gy is not None:
             gy, d.ldgy = _rows(gy)
             d.gy = gy.data_ptr()
@@ -225,28 +229,25 @@ class _NormFn(torch.autograd.Function):
             gh, d.ldgh = _rows(gh)
             d.gh = gh.data_ptr()
         h, d.ldh = _rows(h)
-        d.h = h.data_ptr()
+        d.h, d.rstd = h.data_ptr(), rstd.data_ptr()
         if w is not None:
             w = w.contiguous()
             d.weight = w.data_ptr()
-        d.rstd, d.span = rstd.data_ptr(), 1
-        drop = ctx.drop
         g_res = g_x = g_w = ws = None
-        if need[1] or (need[0] and drop is None):
+        if need[1] or not ctx.drop:
             g_res = torch.empty(h.shape, dtype=h.dtype, device=dev)
             d.g_res, d.ldgr = g_res.data_ptr(), d.cols
-        if drop is None:
+        if not ctx.drop:
             g_x = g_res if need[0] else None
         elif need[0]:
             g_x = torch.empty(h.shape, dtype=h.dtype, device=dev)
             d.g_x, d.ldgx = g_x.data_ptr(), d.cols
-            d.p, d.span, _, d.seed, d.offset = drop
             if dev_seed is not None:
                 d.seed_dev = dev_seed.data_ptr()
         if need[2]:
             g_w = torch.empty(w.shape, dtype=torch.float32, device=dev)
             d.g_w = g_w.data_ptr()
-            ws = torch.empty(max(1, lib.uncl_rmsnorm_backward_workspace_bytes(d.rows, d.cols)), dtype=torch.uint8, device=dev)
+            ws = torch.empty(lib.uncl_rmsnorm_backward_workspace_bytes(d.rows, d.cols), dtype=torch.uint8, device=dev)
         _call(dev, "uncl_rmsnorm_backward", lib.uncl_rmsnorm_backward, C.byref(d), None if ws is None else ws.data_ptr())
         return g_x, g_res if need[1] else None, g_w, None, None
 
@@ -264,8 +265,8 @@ def _norm_checks(x, residual, weight, eps):
     return eps
 
 
-def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def _wants_grad(a, b=None, c=None):
+    return torch.is_grad_enabled() and ((a is not None and a.requires_grad) or (b is not None and b.requires_grad) or (c is not None and c.requires_grad))
 
 
 def rms_norm(x, weight=None, eps=1e-6):
@@ -314,11 +315,12 @@ def _no_grad(what, *ts):
 
 def _empty8(rows, cols, fmt, block, dev):
     """rows on 16-byte borders; row scales lie block by block, as the product reads them"""
-    pitch = -(-cols // 16) * 16
-    data = torch.empty(rows, pitch, dtype=torch.uint8, device=dev).view(_F8[fmt])[:, :cols]
-    kb = -(-cols // BLOCK)
-    scale = (torch.empty(kb, rows, dtype=torch.float32, device=dev).t() if block == "row"
-             else torch.empty(-(-rows // BLOCK), kb, dtype=torch.float32, device=dev))
+    pitch, kb = (cols + 15) & ~15, (cols + 127) // BLOCK
+    data = torch.empty(rows, pitch, dtype=_F8[fmt], device=dev)
+    if pitch != cols:
+        data = data[:, :cols]
+    scale = (torch.empty_strided((rows, kb), (1, rows), dtype=torch.float32, device=dev) if block == "row"
+             else torch.empty((rows + 127) // BLOCK, kb, dtype=torch.float32, device=dev))
     return Quant8(data, scale, block)
 
 
@@ -361,20 +363,22 @@ def quantize8(x, block="row", transpose=False, fmt="e4m3"):
 
 
 def _operand(t):
-    """8-bit rows as the product reads them: on 16-byte borders, readable up to the next one behind a row's end"""
-    rows, cols = t.shape
-    room = -(-cols // 16) * 16
-    end = t.storage_offset() + (rows - 1) * t.stride(0) + room
-    if (cols <= 1 or t.stride(1) == 1) and t.stride(0) >= cols and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0 and end <= t.untyped_storage().nbytes():
-        return t
+    """8-bit rows as the product reads them: on 16-byte borders, readable up to the next one behind a row's end; (tensor, pitch)"""
+    (rows, cols), (pitch, step) = t.shape, t.stride()
+    room = (cols + 15) & ~15
+    if (step == 1 or cols == 1) and pitch >= cols and pitch % 16 == 0 and t.data_ptr() % 16 == 0 and (
+            pitch >= room and t.storage_offset() + (rows - 1) * pitch + room <= t.untyped_storage().nbytes()):
+        return t, pitch
     out = torch.zeros(rows, room, dtype=torch.uint8, device=t.device)
     out[:, :cols] = t.view(torch.uint8) if t.is_contiguous() else t.contiguous().view(torch.uint8)
-    return out.view(t.dtype)[:, :cols]
+    return out.view(t.dtype)[:, :cols], room
 
 
 def _scale(t, most=1 << 20):
-    """block scales with rows as near as the product wants them: within 32-bit offsets, or neighbours"""
-    return t if (1 if most == 1 else 0) <= t.stride(0) <= most else t.t().contiguous().t()
+    """block scales with rows as near as the product wants them, within 32-bit offsets or neighbours; (tensor, its two strides)"""
+    if not (1 if most == 1 else 0) <= t.stride(0) <= most:
+        t = t.t().contiguous().t()
+    return t, t.stride()
 
 
 def _quant_checks(q, what, blocks, dtypes):
@@ -382,11 +386,12 @@ def _quant_checks(q, what, blocks, dtypes):
         raise TypeError("uncltmo_amd: %s must be a Quant8 (see quantize8), got %s" % (what, type(q).__name__))
     if q.block not in blocks:
         raise ValueError("uncltmo_amd: %s must have blocks by %s, got %r" % (what, " or ".join(blocks), q.block))
-    _need(q.data, what + ".data", dtypes)
-    if q.data.dim() != 2:
-        raise ValueError("uncltmo_amd: %s.data must be a matrix, got shape %s" % (what, tuple(q.data.shape)))
-    r, c = q.data.shape
-    _need(q.scale, what + ".scale", (torch.float32,), ((r if q.block == "row" else -(-r // BLOCK)), -(-c // BLOCK)), q.data.device)
+    data = _need(q.data, what + ".data", dtypes)
+    if data.dim() != 2:
+        raise ValueError("uncltmo_amd: %s.data must be a matrix, got shape %s" % (what, tuple(data.shape)))
+    r, c = data.shape
+    _need(q.scale, what + ".scale", (torch.float32,), (r if q.block == "row" else (r + 127) // BLOCK, (c + 127) // BLOCK), data.device)
+    return data
 
 
 def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16, out=None):
@@ -394,12 +399,12 @@ def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16
     in out_dtype, sums in fp32.
     bias: fp32 (N); act: none / relu / lrelu / gelu / sigmoid / tanh / msig; residual: (M, N) in out_dtype.  out: a tensor of that shape and
     type to write (the residual itself among them).  No gradient: linear8 is the form for training."""
-    _quant_checks(a, "a", ("row",), tuple(_F8_CODE))
-    _quant_checks(b, "b", ("tile", "row"), (torch.float8_e4m3fn,))
-    dev = a.data.device
-    (m, k), (n, kb) = a.data.shape, b.data.shape
-    if k != kb or b.data.device != dev:
-        raise ValueError("uncltmo_amd: a is (M, K) = %s on %s, b (N, K) = %s on %s" % ((m, k), dev, (n, kb), b.data.device))
+    ad = _quant_checks(a, "a", ("row",), _F8_TYPES)
+    bd = _quant_checks(b, "b", ("tile", "row"), (torch.float8_e4m3fn,))
+    dev = ad.device
+    (m, k), (n, kb) = ad.shape, bd.shape
+    if k != kb or bd.device != dev:
+        raise ValueError("uncltmo_amd: a is (M, K) = %s on %s, b (N, K) = %s on %s" % ((m, k), dev, (n, kb), bd.device))
     if k == 0:
         raise ValueError("uncltmo_amd: matmul8 needs a common axis of at least one element")
     if act not in _ACT:
@@ -414,21 +419,23 @@ def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16
         _need(residual, "residual", (out_dtype,), (m, n), dev)
     _no_grad("matmul8", bias, residual, out)
     if out is None:
-        out = torch.empty(m, n, dtype=out_dtype, device=dev)
+        out, ldo = torch.empty(m, n, dtype=out_dtype, device=dev), n
     else:
         _need(out, "out", (out_dtype,), (m, n), dev)
-        if _pitch(out) is None:
+        ldo = _pitch(out)
+        if ldo is None:
             raise ValueError("uncltmo_amd: out must have rows of neighbouring elements, got strides %s" % (out.stride(),))
     if m == 0 or n == 0:
         return out
     if residual is not None:
         residual, d.ldr = _rows(residual)
         d.res = residual.data_ptr()
-    ad, bd, sa, sb = _operand(a.data), _operand(b.data), _scale(a.scale), _scale(b.scale, 1 if b.block == "row" else 1 << 20)
-    d.M, d.N, d.K, d.a_fmt, d.b_fmt, d.b_tile = m, n, k, _F8_CODE[ad.dtype], _F8_CODE[bd.dtype], int(b.block == "tile")
-    d.a, d.lda, d.a_scale, d.a_scale_row, d.a_scale_block = ad.data_ptr(), ad.stride(0), sa.data_ptr(), sa.stride(0), sa.stride(1)
-    d.b, d.ldb, d.b_scale, d.b_scale_row, d.b_scale_block = bd.data_ptr(), bd.stride(0), sb.data_ptr(), sb.stride(0), sb.stride(1)
-    d.act, d.out_dtype, d.out, d.ldo = _ACT[act], _CODE[out_dtype], out.data_ptr(), _pitch(out)
+    tile = b.block == "tile"
+    (ad, lda), (bd, ldb), (sa, sas), (sb, sbs) = _operand(ad), _operand(bd), _scale(a.scale), _scale(b.scale, 1 << 20 if tile else 1)
+    d.M, d.N, d.K, d.a_fmt, d.b_fmt, d.b_tile = m, n, k, _F8_CODE[ad.dtype], _hip.E4M3, tile
+    d.a, d.lda, d.a_scale, (d.a_scale_row, d.a_scale_block) = ad.data_ptr(), lda, sa.data_ptr(), sas
+    d.b, d.ldb, d.b_scale, (d.b_scale_row, d.b_scale_block) = bd.data_ptr(), ldb, sb.data_ptr(), sbs
+    d.act, d.out_dtype, d.out, d.ldo = _ACT[act], _CODE[out_dtype], out.data_ptr(), ldo
     lib = _hip.lib()
     size = lib.uncl_matmul8_workspace_bytes(m, n, k) if m > 64 else 0
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
