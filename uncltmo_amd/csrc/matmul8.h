@@ -71,16 +71,17 @@ __device__ __forceinline__ void mm_block(const Wide (&b)[TN], const Wide& a, f32
     for (int j = 0; j < TN; ++j) d[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j].v[i], a.v[i], d[j], 0, 0, 0);
 }
 
-// erf by Abramowitz and Stegun 7.1.26 (off by at most 1.5e-7): the library's erff took half of a short product's time
+// x Phi(x) = max(x, 0) - |x| (1 - Phi(|x|)), the tail by Abramowitz and Stegun 7.1.26 (erf off by at most 1.5e-7): the library's erff took
+// half of a short product's time
 __device__ __forceinline__ float mm_gelu(float x) {
-  const float z = __builtin_fabsf(x) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, z, 1.f));
-  float q = fmaf(t, 1.061405429f, -1.453152027f);
-  q = fmaf(t, q, 1.421413741f);
-  q = fmaf(t, q, -0.284496736f);
-  q = fmaf(t, q, 0.254829592f);
-  const float e = q * t * __builtin_amdgcn_exp2f(z * z * -1.44269504088896341f);      // 1 - erf(z)
-  return x * (x > 0.f ? 1.f - 0.5f * e : 0.5f * e);
+  const float a = __builtin_fabsf(x);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, a, 1.f));
+  float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  q = fmaf(t, q, 0.5f * 1.421413741f);
+  q = fmaf(t, q, 0.5f * -0.284496736f);
+  q = fmaf(t, q, 0.5f * 0.254829592f);
+  const float e = __builtin_amdgcn_exp2f(x * x * (-0.5f * 1.44269504088896341f));
+  return fmaxf(x, 0.f) - a * (q * t * e);
 }
 // the rarer activations, one copy of their code
 __device__ __attribute__((noinline)) float mm_act_rare(float v, int act) { return uncl_act(v, act); }
@@ -331,14 +332,15 @@ __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(
 
 // Time goes by rounds of workgroups over the 256 CUs.  256 x 256 tiles (8-bit instruction, b scaled by tiles) work one to a CU, a round of
 // them is four units of 256 x 128 x 128; 128 x 128 ones two to a CU, two units a round, a tenth slower a unit (8192 x 4096 x 4096: 129
-// against 146 us; 4099 x 4096 x 2048, 8 units against 6: 65 against 53 us).  64 x 64 tiles where 128 x 128 ones are at most one a CU (512 x
+// against 146 us; 4099 x 4096 x 2048, 8 units against 6: 65 against 53 us; a short K leaves nothing to hide the epilogue behind but another
+// workgroup: 28800 x 1024 x 256 with GELU 35.8 against 33.4 us).  64 x 64 tiles where 128 x 128 ones are at most one a CU (512 x
 // 4096 x 4096: 19 against 27 us; 2048 x 2048 x 2048 17.2 against 17.7).
 template <typename T, int FA, bool BT, bool EXACT>
 int launch_tiles(const MmArgs& p, hipStream_t s) {
   auto tiles = [&](int t) { return (long long)((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
   const long long t128 = tiles(128);
   if constexpr (BT && !EXACT) {
-    if (t128 > 256 && 40 * ((tiles(256) + 255) / 256) <= 22 * ((t128 + 511) / 512)) {
+    if (t128 > 256 && p.KB >= 6 && 40 * ((tiles(256) + 255) / 256) <= 22 * ((t128 + 511) / 512)) {
       mm_tile_kernel<T, FA, BT, EXACT, 256, 256, 2, 4><<<(unsigned)tiles(256), 512, 0, s>>>(p);
       UNCL_CHECK_LAUNCH();
       return UNCL_OK;
