@@ -17,6 +17,8 @@
 #include "matmul8_args.h"
 #include "row_ops.h"
 
+#include <type_traits>
+
 // the tiled kernels, one file for each type of result: bf16 through the 8-bit instruction, fp16 and fp32 through the bf16 one
 int mm_tiles_bf16(const MmArgs& p, int a_fmt, bool b_tile, hipStream_t s);
 int mm_tiles_f16(const MmArgs& p, int a_fmt, bool b_tile, hipStream_t s);
@@ -111,13 +113,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mm_buffer(const void* p, long 
   const long long n = (rows - 1) * pitch + len;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)(n < 0x7fffffffll ? n : 0x7fffffffll), 0x00020000);
 }
-__device__ __forceinline__ float mm_buffer_f32(__amdgpu_buffer_rsrc_t r, int offset) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, offset, 0, 0));
-}
 
 // ---- tiles ---------------------------------------------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves owns BM x BN outputs; a stage of LDS holds 128 bytes of each of its BM + BN rows, two stages.  Rows
-// come in by asynchronous 16-byte loads straight to LDS, a block ahead of the products (the scales likewise, to registers): one barrier
+// come in by asynchronous 16-byte loads straight to LDS, a block ahead of the products, and the block's scales with them: one barrier
 // a block says both that this block has arrived and that nobody reads the stage that the next one overwrites.  Chunk c of row r lies at
 // position c ^ mm_turn(r), so that the rows that a part of a wave reads at once fall on different banks (no conflicts are counted).  The loads write LDS in
 // lane order, hence the swizzle is in the lane's global address.  Rows behind M or N are out of the buffers' bounds (their results are not
@@ -131,7 +130,9 @@ template <typename T, int FA, bool BT, bool EXACT, int BM, int BN, int WM, int W
 __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(const MmArgs p) {
   constexpr int NT = WM * WN * 64, TM = BM / WM / 16, TN = BN / WN / 16, STAGE = (BM + BN) * 128;
   constexpr int LA = BM * 8 / NT, LB = BN * 8 / NT;         // 16-byte loads a thread and stage
-  __shared__ __align__(16) unsigned char lds[2 * STAGE];
+  constexpr int SB = BT ? (BN > 128 ? BN / 128 : 1) : BN / 64;   // waves that fetch b's scales
+  constexpr int SCALES = (BM + SB * 64) * 4;                 // a block's scales, behind the two stages
+  __shared__ __align__(16) unsigned char lds[2 * (STAGE + SCALES)];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
   const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, total = tm * tn;
   int id = blockIdx.x;
@@ -149,13 +150,14 @@ __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(
   const int va = (wave * 8 + lr) * (int)p.lda + lc * 16, vb = (wave * 8 + lr) * (int)p.ldb + lc * 16;
   const int sta = (NT / 8) * (int)p.lda, stb = (NT / 8) * (int)p.ldb;
   typedef __attribute__((address_space(3))) void* lptr;
-  auto fetch = [&](int kb) {
+  auto fetch_one = [&](int kb, int x) {                      // the x-th of a wave's LA + LB loads of a block
     unsigned char* base = lds + (kb & 1) * STAGE + wave * 1024;
+    if (x < LA) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lptr)(base + x * NT * 16), 16, va + x * sta, kb * 128, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lptr)(base + BM * 128 + (x - LA) * NT * 16), 16, vb + (x - LA) * stb, kb * 128, 0, 0);
+  };
+  auto fetch = [&](int kb) {
 #pragma unroll
-    for (int i = 0; i < LA; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lptr)(base + i * NT * 16), 16, va + i * sta, kb * 128, 0, 0);
-#pragma unroll
-    for (int i = 0; i < LB; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lptr)(base + BM * 128 + i * NT * 16), 16, vb + i * stb, kb * 128, 0, 0);
+    for (int x = 0; x < LA + LB; ++x) fetch_one(kb, x);
   };
 
   f32x4 acc[TN][TM];
@@ -164,110 +166,191 @@ __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(
 #pragma unroll
     for (int i = 0; i < TM; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int q = lane & 15, g = lane >> 4;
-  const int mb = m0 + wm * TM * 16, nb = n0 + wn * TN * 16;   // the wave's columns lie inside one 128-column tile of b's scales
-  const float *sap = p.sa + (long long)m0 * p.sa_row, *sbp = p.sb + (BT ? ((nb < p.N ? nb : p.N - 1) >> 7) * p.sb_row : n0);
-  const int so = (mb - m0 + q) * (int)p.sa_row * 4, sno = (nb - n0 + g * 4) * 4;
-  float sm_next[TM], sb_next = 1.f;
-  f32x4 sn_next[BT ? 1 : TN];
+  const int mb = m0 + wm * TM * 16, nb = n0 + wn * TN * 16;
+  const float* sap = p.sa + (long long)m0 * p.sa_row;
+  // one wave for each 64 of a's rows, and for each 64 of b's columns or each tile of b's scales (64 copies of it)
   auto fetch_scales = [&](int kb) {
-    const __amdgpu_buffer_rsrc_t rs = mm_buffer(sap + kb * p.sa_blk, p.M - m0, p.sa_row * 4, 4);
-#pragma unroll
-    for (int i = 0; i < TM; ++i) sm_next[i] = mm_buffer_f32(rs, so + i * 64 * (int)p.sa_row);
-    if constexpr (BT) {
-      sb_next = sbp[kb * p.sb_blk];
-    } else {
-      const __amdgpu_buffer_rsrc_t rn = mm_buffer(sbp + kb * p.sb_blk, p.N - n0, 4, 4);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) sn_next[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rn, sno + j * 64, 0, 0));
+    unsigned char* to = lds + 2 * STAGE + (kb & 1) * SCALES + wave * 256;
+    const int x = wave - BM / 64;
+    if (x < 0) {
+      const __amdgpu_buffer_rsrc_t r = mm_buffer(sap + kb * p.sa_blk, p.M - m0, p.sa_row * 4, 4);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)to, 4, (wave * 64 + lane) * (int)p.sa_row * 4, 0, 0, 0);
+    } else if (x < SB) {
+      if constexpr (BT) {
+        const int last_tile = (p.N - 1) >> 7, tile = (n0 >> 7) + x;
+        const __amdgpu_buffer_rsrc_t r = mm_buffer(p.sb + (tile < last_tile ? tile : last_tile) * p.sb_row + kb * p.sb_blk, 1, 4, 4);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)to, 4, 0, 0, 0, 0);
+      } else {
+        const __amdgpu_buffer_rsrc_t r = mm_buffer(p.sb + n0 + kb * p.sb_blk, p.N - n0, 4, 4);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr)to, 4, (x * 64 + lane) * 4, 0, 0, 0);
+      }
     }
   };
+  float sb = 1.f;                                            // b's scale (BT), of the block at work
+  f32x4 sn[BT ? 1 : TN];                                     // or those of the lane's columns
+  auto scales = [&](int kb) { return reinterpret_cast<const float*>(lds + 2 * STAGE + (kb & 1) * SCALES); };
+  auto take_scales = [&](int kb) {
+    if constexpr (BT) sb = scales(kb)[BM + ((wn * TN * 16) >> 7) * 64 + lane];
+    else
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sn[j] = *reinterpret_cast<const f32x4*>(scales(kb) + BM + wn * TN * 16 + g * 4 + j * 16);
+  };
+  auto scale_a = [&](int kb, int i) { return scales(kb)[(wm * TM + i) * 16 + q]; };
 
   int k0 = 0, k1 = p.KB;
   if constexpr (BM == 64)
     if (p.part) { k0 = blockIdx.y * p.per; k1 = k0 + p.per < p.KB ? k0 + p.per : p.KB; }
   fetch(k0);
   fetch_scales(k0);
-  for (int kb = k0; kb < k1; ++kb) {
+  auto stage = [&](int kb) { return lds + (kb & 1) * STAGE; };
+  // block kb has arrived (and nobody reads the other stage any more); a short last block: what lies behind K is cleared
+  auto arrive = [&](int kb) {
     mm_arrive();
-    float sm[TM];
-    f32x4 sn[BT ? 1 : TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) sm[i] = sm_next[i] * sb_next;
-    if constexpr (!BT)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) sn[j] = sn_next[j];
-    if (kb + 1 < k1) {
-      fetch(kb + 1);
-      fetch_scales(kb + 1);
-    }
-    unsigned char* st = lds + (kb & 1) * STAGE;
     const int have = p.K - kb * 128;
-    if (have < 128) {                                        // the last block is short: clear what lies behind K
-      for (int t = threadIdx.x; t < (BM + BN) * 8; t += NT) {
-        const int r = t >> 3, c = t & 7;
-        unsigned char* at = st + r * 128 + ((c ^ mm_turn(r)) << 4);
-        const int keep = have - c * 16;
-        if (keep <= 0) *reinterpret_cast<i32x4*>(at) = i32x4{0, 0, 0, 0};
-        else
-          for (int k = keep; k < 16; ++k) at[k] = 0;
-      }
-      mm_arrive();
+    if (have >= 128) return;
+    for (int t = threadIdx.x; t < (BM + BN) * 8; t += NT) {
+      const int r = t >> 3, c = t & 7;
+      unsigned char* at = stage(kb) + r * 128 + ((c ^ mm_turn(r)) << 4);
+      const int keep = have - c * 16;
+      if (keep <= 0) *reinterpret_cast<i32x4*>(at) = i32x4{0, 0, 0, 0};
+      else
+        for (int k = keep; k < 16; ++k) at[k] = 0;
     }
-    auto frag = [&](int row) {
-      const unsigned char* r = st + row * 128;
-      const i32x4 lo = *reinterpret_cast<const i32x4*>(r + ((g ^ mm_turn(row)) << 4));
-      const i32x4 hi = *reinterpret_cast<const i32x4*>(r + (((g + 4) ^ mm_turn(row)) << 4));
-      return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    mm_arrive();
+  };
+  auto frag = [&](const unsigned char* st, int row) {
+    const unsigned char* r = st + row * 128;
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(r + ((g ^ mm_turn(row)) << 4));
+    const i32x4 hi = *reinterpret_cast<const i32x4*>(r + (((g + 4) ^ mm_turn(row)) << 4));
+    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  const int rowa = wm * TM * 16 + q, rowb = BM + wn * TN * 16 + q;
+  // the products of a's rows i run while those of rows i - 1 join their sums: a matrix instruction's result is never waited for
+  f32x4 t[2][TN];
+  auto join_one = [&](int i, int j, float scale) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(t[i & 1][j][e], BT ? scale : scale * sn[BT ? 0 : j][e], acc[j][i][e]);
+  };
+  auto join = [&](int i, float scale) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) join_one(i, j, scale);
+  };
+  if constexpr (BM == 256) {
+    // One workgroup a CU: nobody else works while this one waits.  The next block's arrival is waited for before this block's last
+    // products, whose time its first LDS reads then have; its loads are spread over the first half of this block's products (64 at once
+    // kept the waves from issuing anything else); the last sums join in the next block.  8192 x 8192 x 8192: 468 -> 441 us; the smaller
+    // tiles, two to four workgroups a CU, lost 5 - 10 % by it.
+    i32x8 fb[TN], fa[2];
+    float sm[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < TN; ++j) t[(TM - 1) & 1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](int i, int j) {
+      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+      t[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[i & 1], z, UNCL_E4M3 - 1, FA - 1, 0, 0, 0, 0);
     };
-    // the products of a's rows i run while those of rows i - 1 join their sums: a matrix instruction's result is never waited for
-    decltype(mm_frag<UNCL_E4M3, EXACT>(i32x8{})) fb[TN], fa[2];
-    fa[0] = mm_frag<FA, EXACT>(frag(wm * TM * 16 + q));
+    constexpr int HALF = TM / 2, EACH = (LA + LB + HALF - 1) / HALF;     // loads of the next block: spread over the first half
+    auto all_but_last = [&](int kb, auto more) {
+      const unsigned char* st = stage(kb);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) fb[j] = mm_frag<UNCL_E4M3, EXACT>(frag(BM + (wn * TN + j) * 16 + q));
-    f32x4 t[2][TN];
+      for (int i = 0; i + 1 < TM; ++i) {
+        fa[(i + 1) & 1] = frag(st, rowa + (i + 1) * 16);
 #pragma unroll
-    for (int i = 0; i <= TM; ++i) {
-      i32x8 raw;
-      if (i + 1 < TM) raw = frag((wm * TM + i + 1) * 16 + q);
-      if (i < TM) mm_block<FA, TN>(fb, fa[i & 1], t[i & 1]);
-      if (i > 0) {
+        for (int j = 0; j < TN; ++j) multiply(i, j);
+        join((i + TM - 1) % TM, i == 0 ? sm[1] : sm[(i + 1) & 1] * sb);           // (rows TM - 1: of the last block, scaled already)
+        sm[(i + 1) & 1] = scale_a(kb, i + 1);
+        if constexpr (more)
+#pragma unroll
+          for (int x = i * EACH; x < (i + 1) * EACH && x < LA + LB; ++x) fetch_one(kb + 1, x);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                        // LDS reads of the next rows
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                      // a matrix instruction,
+          __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);                      // the last rows' multiply-adds under it
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // what has been joined stays joined: left to itself the compiler moves all multiply-adds behind the next branch, their operands with them
+    auto pin = [&]() {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
+          if (i != TM - 2) asm volatile("" : "+v"(acc[j][i]));
+    };
+    arrive(k0);
+    fa[0] = frag(stage(k0), rowa);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][i - 1][e] = fmaf(t[(i - 1) & 1][j][e], BT ? sm[i - 1] : sm[i - 1] * sn[BT ? 0 : j][e], acc[j][i - 1][e]);
-      }
-      if (i + 1 < TM) fa[(i + 1) & 1] = mm_frag<FA, EXACT>(raw);
-      if constexpr (!EXACT) {
-        if (i == 0) {                                                             // each product as soon as its operands are read
-          __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          }
-        } else if (i < TM) {
-          if (i + 1 < TM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);      // LDS reads of the next rows
-#pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                    // a matrix instruction,
-            __builtin_amdgcn_sched_group_barrier(0x002, BT ? 4 : 8, 0);           // the last rows' multiply-adds under it
-          }
-        }
-      } else if (i < TM) {
-        if (i + 1 < TM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-#pragma unroll
-        for (int j = 0; j < 4 * TN; ++j) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x002, BT ? 2 : 3, 0);
-        }
-      }
+    for (int j = 0; j < TN; ++j) fb[j] = frag(stage(k0), rowb + j * 16);
+    take_scales(k0);
+    sm[0] = scale_a(k0, 0);
+    for (int kb = k0; kb + 1 < k1; ++kb) {
+      fetch_scales(kb + 1);
+      all_but_last(kb, std::true_type{});
+      pin();
+      arrive(kb + 1);
+      const unsigned char* next = stage(kb + 1);
+      sm[0] *= sb;
+      sm[1] *= sb;
       __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {                                              // (in this order: the next operand takes the last one's registers)
+        multiply(TM - 1, j);
+        __builtin_amdgcn_sched_barrier(0);
+        fb[j] = frag(next, rowb + j * 16);
+        join_one(TM - 2, j, sm[0]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      fa[0] = frag(next, rowa);
+      take_scales(kb + 1);
+      sm[0] = scale_a(kb + 1, 0);
+    }
+    all_but_last(k1 - 1, std::false_type{});
+    pin();
+#pragma unroll
+    for (int j = 0; j < TN; ++j) multiply(TM - 1, j);
+    join(TM - 2, sm[0] * sb);
+    join(TM - 1, sm[1] * sb);
+  } else {
+    for (int kb = k0; kb < k1; ++kb) {
+      arrive(kb);
+      take_scales(kb);
+      if (kb + 1 < k1) {
+        fetch(kb + 1);
+        fetch_scales(kb + 1);
+      }
+      const unsigned char* st = stage(kb);
+      decltype(mm_frag<UNCL_E4M3, EXACT>(i32x8{})) fb[TN], fa[2];
+      fa[0] = mm_frag<FA, EXACT>(frag(st, rowa));
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[j] = mm_frag<UNCL_E4M3, EXACT>(frag(st, rowb + j * 16));
+      float sm[2];
+#pragma unroll
+      for (int i = 0; i <= TM; ++i) {
+        i32x8 raw;
+        if (i + 1 < TM) raw = frag(st, rowa + (i + 1) * 16);
+        if (i < TM) sm[i & 1] = scale_a(kb, i);
+        if (i < TM) mm_block<FA, TN>(fb, fa[i & 1], t[i & 1]);
+        if (i > 0) join(i - 1, BT ? sm[(i - 1) & 1] * sb : sm[(i - 1) & 1]);
+        if (i + 1 < TM) fa[(i + 1) & 1] = mm_frag<FA, EXACT>(raw);
+        if (i < TM) {
+          if (i + 1 < TM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+          for (int j = 0; j < (EXACT ? 4 : 1) * TN; ++j) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, EXACT ? (BT ? 2 : 3) : 8, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
   // A lane's results are four columns of sixteen different rows: they turn round in LDS, 32 rows of the wave at a time, so that eight (or
   // four) lanes hold one row's columns and memory sees whole lines.  Each wave has its own part of LDS, whose operations stay in order.
   constexpr int COLS = TN * 16, PITCH = COLS + 4, LPR = COLS / 8, RPP = 64 / LPR, PASSES = 32 / RPP;
-  static_assert(WM * WN * 32 * PITCH * 4 <= 2 * STAGE && TM % 2 == 0, "the turned rows fit where the stages were");
+  static_assert(BM < 256 || (BT && !EXACT), "the largest tiles are built for the 8-bit instruction and b scaled by tiles");
+  static_assert(WM * WN * 32 * PITCH * 4 <= 2 * STAGE && TM % 2 == 0 && BM / 64 + SB <= WM * WN, "the turned rows fit where the stages were");
   mm_arrive();
   float* w = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
   const int r0 = lane / LPR, c0 = (lane % LPR) * 8, n = nb + c0, left = p.N - n;
