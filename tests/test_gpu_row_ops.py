@@ -340,7 +340,7 @@ def test_product_outputs(dtype, m, n):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
-@pytest.mark.parametrize("m,n,k", [(2100, 2050, 384), (28800, 256, 256), (4101, 3500, 1100), (300, 33000, 1024)])
+@pytest.mark.parametrize("m,n,k", [(2100, 2050, 384), (28800, 256, 256), (4101, 3500, 1100), (300, 33000, 1024), (4099, 4096, 2048), (4099, 2048, 4096)])
 def test_product_of_many_tiles(m, n, k, dtype):
     """the large shapes against a 64-bit product on the GPU of what the operands stand for"""
     _, a = operand(m, k, "row")

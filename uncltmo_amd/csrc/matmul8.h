@@ -413,24 +413,14 @@ __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(
   }
 }
 
-// Time goes by rounds of workgroups over the 256 CUs.  256 x 256 tiles (8-bit instruction, b scaled by tiles) work one to a CU, a round of
-// them is four units of 256 x 128 x 128; 128 x 128 ones two to a CU, two units a round, a tenth slower a unit (8192 x 4096 x 4096: 129
-// against 146 us; 4099 x 4096 x 2048, 8 units against 6: 65 against 53 us; a short K leaves nothing to hide the epilogue behind but another
-// workgroup: 28800 x 1024 x 256 with GELU 35.8 against 33.4 us).  64 x 64 tiles where 128 x 128 ones are at most one a CU (512 x
-// 4096 x 4096: 19 against 27 us; 2048 x 2048 x 2048 17.2 against 17.7).
 template <typename T, int FA, bool BT, bool EXACT>
 int launch_tiles(const MmArgs& p, hipStream_t s) {
-  auto tiles = [&](int t) { return (long long)((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
-  const long long t128 = tiles(128);
-  if constexpr (BT && !EXACT) {
-    if (t128 > 256 && p.KB >= 6 && 40 * ((tiles(256) + 255) / 256) <= 22 * ((t128 + 511) / 512)) {
-      mm_tile_kernel<T, FA, BT, EXACT, 256, 256, 2, 4><<<(unsigned)tiles(256), 512, 0, s>>>(p);
-      UNCL_CHECK_LAUNCH();
-      return UNCL_OK;
-    }
-  }
-  if (t128 > 256) mm_tile_kernel<T, FA, BT, EXACT, 128, 128, 2, 2><<<(unsigned)t128, 256, 0, s>>>(p);
-  else mm_tile_kernel<T, FA, BT, EXACT, 64, 64, 2, 2><<<dim3((unsigned)tiles(64), p.part ? (p.KB + p.per - 1) / p.per : 1), 256, 0, s>>>(p);
+  const MmPlan plan = mm_plan(p.M, p.N, p.KB, BT && !EXACT);
+  if constexpr (BT && !EXACT)
+    if (plan.tile == 256) mm_tile_kernel<T, FA, BT, EXACT, 256, 256, 2, 4><<<(unsigned)mm_tiles(p.M, p.N, 256), 512, 0, s>>>(p);
+  if (plan.tile == 128) mm_tile_kernel<T, FA, BT, EXACT, 128, 128, 2, 2><<<(unsigned)mm_tiles(p.M, p.N, 128), 256, 0, s>>>(p);
+  if (plan.tile == 64)
+    mm_tile_kernel<T, FA, BT, EXACT, 64, 64, 2, 2><<<dim3((unsigned)mm_tiles(p.M, p.N, 64), p.part ? (p.KB + p.per - 1) / p.per : 1), 256, 0, s>>>(p);
   UNCL_CHECK_LAUNCH();
   return UNCL_OK;
 }

@@ -14,9 +14,27 @@ struct MmArgs {
   int per;
 };
 
+static inline long long mm_tiles(int M, int N, int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); }
+
+// Which tiles, and their time in tenths of a round of 256 x 128 x 128 outputs.  Time goes by rounds of workgroups over the 256 CUs.  256 x 256
+// tiles (8-bit instruction, b scaled by tiles) work one to a CU, four units a round; 128 x 128 ones two to a CU, two units a round, a
+// tenth slower a unit (8192 x 4096 x 4096: 124 against 146 us; 4099 x 4096 x 2048, 8 units against 6: 65 against 51 us; a short K leaves
+// nothing to hide the epilogue behind but another workgroup: 28800 x 1024 x 256 with GELU 35.8 against 33.4 us).  64 x 64 tiles, four to a CU,
+// where 128 x 128 ones are at most one a CU (512 x 4096 x 4096: 19 against 27 us; 2048 x 2048 x 2048 17.2 against 17.7).
+struct MmPlan {
+  int tile;
+  long long units;
+};
+static inline MmPlan mm_plan(int M, int N, int kb, bool large) {
+  const long long t128 = mm_tiles(M, N, 128), u128 = 22 * ((t128 + 511) / 512), u256 = 40 * ((mm_tiles(M, N, 256) + 255) / 256);
+  if (t128 <= 256) return {64, 12 * ((mm_tiles(M, N, 64) + 1023) / 1024)};
+  if (large && kb >= 6 && u256 <= u128) return {256, u256};
+  return {128, u128};
+}
+
 // workgroups that share a tile's K: 1, or enough for two a CU where 64 x 64 tiles leave CUs idle, at least four blocks each
 static inline int mm_splits(int M, int N, int K) {
-  const long long t = (long long)((M + 63) / 64) * ((N + 63) / 64);
+  const long long t = mm_tiles(M, N, 64);
   const int kb = (K + 127) / 128;
   if (M <= 64 || t >= 256 || kb < 8) return 1;
   long long s = (512 + t - 1) / t;
