@@ -716,7 +716,7 @@ int uncl_optical_flow(const float* img_to_align, const float* img_source, int H,
 
 /* ------------------------------------------------------------------------------------------------------
  * Operators on rows of channels.  A row is one pixel or graph node of a channel-last tensor: `cols` consecutive elements, rows `ld*`
- * elements apart (ld >= cols, any alignment of the element type).  Elements are fp32, bf16 or fp16 (`dtype`); sums, statistics and
+ * elements apart (ld >= cols, any alignment of the element type); up to 2^32 rows and 2^30 columns.  Elements are fp32, bf16 or fp16 (`dtype`); sums, statistics and
  * weight gradients are fp32.  The reference composes its bottleneck of DropPath, residual additions and 1x1 convolutions
  * (Unet_singleFrame.py:25-41, torch_vertex.py:181-227); these are the forms a wider bottleneck needs beside uncl_scale_rows,
  * uncl_inorm_act / uncl_bnorm_act and uncl_conv_igemm.  Calls with no elements return UNCL_OK and launch nothing.

@@ -217,11 +217,29 @@ def test_norm_views_empty_and_one_dimension(dtype):
         assert gx.shape == torch.Size(shape) and int(gw.count_nonzero()) == 0
 
 
-def test_norm_of_a_row_with_nan_leaves_the_others():
-    x = rnd(9, 64)
+@pytest.mark.parametrize("cols", [64, 16400])
+def test_norm_of_a_row_with_nan_leaves_the_others(cols):
+    x = rnd(9, cols)
     x[4, 7] = float("nan")
     y = row_ops.rms_norm(x.cuda()).cpu()
     assert torch.isnan(y[4]).all() and torch.isfinite(y[[0, 1, 2, 3, 5, 6, 7, 8]]).all()
+    xs, g = x.cuda().requires_grad_(), rnd(9, cols, seed=1).cuda()
+    _, h = row_ops.add_rms_norm(xs, torch.zeros_like(xs), None, EPS)                   # a gradient of the sum alone passes as it is
+    assert torch.equal(torch.autograd.grad(h, [xs], g)[0], g)
+
+
+def test_gradients_that_are_one_number_everywhere():
+    """a sum's gradient is one element seen from everywhere: rows without a pitch"""
+    x, w = rnd(40, 72).cuda().requires_grad_(), rnd(24, 72, seed=1).cuda().requires_grad_()
+    ones = torch.ones(40, 72, device="cuda")
+    for f, leaves in ((lambda: row_ops.dropout(x, 0.3, 1), [x]), (lambda: row_ops.rms_norm(x), [x]), (lambda: row_ops.linear8(x, w), [x, w])):
+        got = torch.autograd.grad(f().sum(), leaves)
+        want = torch.autograd.grad(f(), leaves, torch.ones_like(f()))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y, h = row_ops.add_rms_norm(x, ones, None, EPS)
+    got, = torch.autograd.grad(y.sum() + 2 * h.sum(), [x])
+    y, h = row_ops.add_rms_norm(x, ones, None, EPS)
+    assert torch.equal(got, torch.autograd.grad([y, h], [x], [ones, 2 * ones])[0])
 
 
 # ---- 8-bit operands --------------------------------------------------------------------------------------------------------------------
@@ -305,6 +323,9 @@ def check_product(m, n, k, block="tile", fa="e4m3", act="none", dtype=torch.floa
         want, tol = want + bv.double(), tol + R.U * (want.abs() + bv.double().abs())
     if act == "relu":
         want = want.clamp_min(0)
+    elif act in ("lrelu", "sigmoid", "tanh", "msig"):             # slopes up to 1; an exponential and a division
+        want = {"lrelu": lambda v: torch.where(v > 0, v, 0.2 * v), "sigmoid": torch.sigmoid, "tanh": torch.tanh, "msig": lambda v: torch.sigmoid(3 * v)}[act](want)
+        tol = tol + 64 * R.U
     elif act == "gelu":
         tol = 1.13 * tol + 16 * R.U * want.abs()                 # the slope is at most 1.13; erf and two products
         want = want * torch.special.ndtr(want)
@@ -329,6 +350,12 @@ def test_product_sizes(m, n, k):
 def test_product_formats(m, block, fa, dtype):
     check_product(m, 200, 400, block, fa, dtype=dtype)
     check_product(m * 9, 1100, 70, block, fa, dtype=dtype)
+
+
+@pytest.mark.parametrize("act", ["lrelu", "sigmoid", "tanh", "msig"])
+@pytest.mark.parametrize("m,k", [(5, 128), (200, 100), (70, 1100)])
+def test_product_rarer_activations(act, m, k):
+    check_product(m, 130, k, act=act, residual=True)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)

@@ -54,7 +54,7 @@ def test_entries_refuse_bad_arguments_before_any_launch():
     def drop(x=p, ldx=8, res=None, ldr=0, y=p, ldy=8, dt=_hip.F32, rows=2, cols=8, prob=0.5, span=1):
         return lib.uncl_dropout(x, ldx, res, ldr, y, ldy, dt, rows, cols, prob, span, None, 1, 2, None)
     for kw in (dict(x=None), dict(y=None), dict(ldx=7), dict(ldy=7), dict(res=p, ldr=7), dict(dt=3), dict(rows=-1), dict(cols=-1), dict(prob=-0.1),
-               dict(prob=1.5), dict(prob=float("nan")), dict(span=0), dict(rows=2 ** 62)):
+               dict(prob=1.5), dict(prob=float("nan")), dict(span=0), dict(rows=2 ** 32 + 1), dict(cols=2 ** 30 + 1, ldx=2 ** 31, ldy=2 ** 31)):
         assert drop(**kw) == bad, kw
     assert drop(rows=0, x=None) == 0 and drop(cols=0, y=None) == 0
 
@@ -65,19 +65,19 @@ def test_entries_refuse_bad_arguments_before_any_launch():
         return C.byref(d)
     base = dict(dtype=_hip.F32, rows=2, cols=8, eps=1e-6, x=p, ldx=8, y=p, ldy=8, span=1)
     for kw in (dict(x=None), dict(y=None), dict(eps=0.0), dict(eps=float("nan")), dict(eps=-1.0), dict(ldx=7), dict(ldy=7), dict(res=p, ldr=7), dict(h=p, ldh=7),
-               dict(dtype=9), dict(rows=-1), dict(y_fmt=3), dict(y_fmt=_hip.E4M3), dict(p=2.0), dict(span=0)):
+               dict(dtype=9), dict(rows=-1), dict(rows=2 ** 32 + 1), dict(cols=2 ** 30 + 1, ldx=2 ** 31, ldy=2 ** 31), dict(y_fmt=3), dict(y_fmt=_hip.E4M3), dict(p=2.0), dict(span=0)):
         assert lib.uncl_rmsnorm(make(_hip.RmsnormDesc, base, **kw), None) == bad, kw
     assert lib.uncl_rmsnorm(None, None) == bad and lib.uncl_rmsnorm(make(_hip.RmsnormDesc, base, rows=0, x=None), None) == 0
     base = dict(dtype=_hip.F32, rows=2, cols=8, h=p, ldh=8, rstd=p, gy=p, ldgy=8, g_res=p, ldgr=8, span=1)
     for kw in (dict(h=None), dict(rstd=None), dict(ldh=7), dict(ldgy=7), dict(gh=p, ldgh=7), dict(ldgr=7), dict(g_x=p, ldgx=7), dict(g_w=p), dict(span=0),
-               dict(p=-1.0), dict(dtype=7), dict(rows=-3)):
+               dict(p=-1.0), dict(dtype=7), dict(rows=-3), dict(rows=2 ** 33), dict(cols=2 ** 30 + 1, ldh=2 ** 31, ldgy=2 ** 31, ldgr=2 ** 31)):
         assert lib.uncl_rmsnorm_backward(make(_hip.RmsnormBwdDesc, base, **kw), None, None) == bad, kw
     assert lib.uncl_rmsnorm_backward(None, None, None) == bad and lib.uncl_rmsnorm_backward_workspace_bytes(0, 8) == 0
     assert lib.uncl_rmsnorm_backward_workspace_bytes(10 ** 7, 40) <= 1024 * 40 * 4
 
     def quant(x=p, dt=_hip.F32, rows=2, cols=8, ldx=8, q=p, ldq=16, fmt=_hip.E4M3, scale=p, tile=0, tr=0):
         return lib.uncl_quant8(x, dt, rows, cols, ldx, q, ldq, fmt, scale, 1, 1, tile, tr, None)
-    for kw in (dict(x=None), dict(q=None), dict(scale=None), dict(dt=4), dict(fmt=0), dict(fmt=3), dict(ldx=7), dict(ldq=7), dict(rows=-1), dict(tr=1, rows=20),
+    for kw in (dict(x=None), dict(q=None), dict(scale=None), dict(dt=4), dict(fmt=0), dict(fmt=3), dict(ldx=7), dict(ldq=7), dict(rows=-1), dict(rows=2 ** 33), dict(cols=2 ** 30 + 1, ldx=2 ** 31, ldq=2 ** 31), dict(tr=1, rows=20),
                dict(tile=1, rows=65535 * 128 + 1), dict(tr=1, rows=65535 * 128 + 1, ldq=2 ** 31)):
         assert quant(**kw) == bad, kw
     assert quant(rows=0, x=None) == 0

@@ -244,7 +244,7 @@ int launch_quant(const QuantArgs& a, int tile, int trans, hipStream_t s) {
 
 extern "C" int uncl_quant8(const void* x, int dtype, long long rows, int cols, long long ldx, void* q, long long ldq, int fmt, float* scale,
                            long long scale_row, long long scale_block, int tile, int transposed, void* stream) {
-  if (!(dtype == UNCL_F32 || uncl_is_h16(dtype)) || (fmt != UNCL_E4M3 && fmt != UNCL_E5M2) || rows < 0 || cols < 0) return UNCL_ERR_ARG;
+  if (!(dtype == UNCL_F32 || uncl_is_h16(dtype)) || (fmt != UNCL_E4M3 && fmt != UNCL_E5M2) || rows < 0 || rows > (1ll << 32) || cols < 0 || cols > (1 << 30)) return UNCL_ERR_ARG;
   if (rows == 0 || cols == 0) return UNCL_OK;
   if (!x || !q || !scale || ldx < cols || ldq < (transposed ? rows : cols)) return UNCL_ERR_ARG;
   if ((tile || transposed) && (rows + 127) / 128 > 65535) return UNCL_ERR_ARG;      // one workgroup a tile, rows along the grid's y

@@ -229,8 +229,9 @@ __global__ __launch_bounds__(256) void norm_back_kernel(const NormBackArgs a) {
     for (int c = 0; c < CH; ++c) {
       const int col = (lane + c * LANES) * 8, n = live ? a.cols - col : 0;
       if (n <= 0) continue;
+      if (a.gy)                                              // (without a gradient of y, 1 / rms counts for nothing, whatever it is)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[c][i] = r * (g[c][i] - n_[c][i] * mean);
+        for (int i = 0; i < 8; ++i) g[c][i] = r * (g[c][i] - n_[c][i] * mean);
       if (a.gh) {
         float q[8];
         ro_load8(reinterpret_cast<const T*>(a.gh) + row * a.ldgh + col, n, q);
@@ -309,6 +310,7 @@ __global__ __launch_bounds__(256) void norm_back_long_kernel(const NormBackArgs 
       if (out && !first) ro_load8(out + col, n, p);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
+        if (!a.gy) continue;
         nv[i] *= r;
         p[i] = fmaf(g[i], nv[i], p[i]);
         g[i] = r * (g[i] * w[i] - nv[i] * mean);
@@ -460,10 +462,9 @@ int launch_norm_back(const NormBackArgs& a, int grid, hipStream_t s) {
 
 bool dtype_ok(int d) { return d == UNCL_F32 || uncl_is_h16(d); }
 
-// flags: span >= 1, and the index of the last group must fit 63 bits (rows * groups)
-bool drop_ok(float p, long long span, long long rows, int cols) {
-  return p >= 0.f && p <= 1.f && span >= 1 && rows <= (1ll << 62) / ((cols + 7) / 8 + 1);
-}
+// columns step in int by up to 2048 behind the last one, flag groups (rows * cols / 8) in 64 bits
+bool extent_ok(long long rows, int cols) { return rows >= 0 && rows <= (1ll << 32) && cols >= 0 && cols <= (1 << 30); }
+bool drop_ok(float p, long long span) { return p >= 0.f && p <= 1.f && span >= 1; }
 
 }  // namespace
 
@@ -476,9 +477,9 @@ int ro_fold_rows(const float* part, int blocks, int cols, float* out, hipStream_
 extern "C" int uncl_dropout(const void* x, long long ldx, const void* res, long long ldr, void* y, long long ldy, int dtype, long long rows,
                             int cols, float p, long long span, const unsigned long long* seed_dev, unsigned long long seed,
                             unsigned long long offset, void* stream) {
-  if (!dtype_ok(dtype) || rows < 0 || cols < 0) return UNCL_ERR_ARG;
+  if (!dtype_ok(dtype) || !extent_ok(rows, cols)) return UNCL_ERR_ARG;
   if (rows == 0 || cols == 0) return UNCL_OK;
-  if (!x || !y || !drop_ok(p, span, rows, cols) || ldx < cols || ldy < cols || (res && ldr < cols)) return UNCL_ERR_ARG;
+  if (!x || !y || !drop_ok(p, span) || ldx < cols || ldy < cols || (res && ldr < cols)) return UNCL_ERR_ARG;
   DropArgs a{x, res, y, rows, ldx, ldr, ldy, cols, (cols + 7) / 8, 0, {seed_dev, seed, offset, span, 0, 1.f}};
   ro_drop_setup(a.drop, p);
   a.lanes = pow2_at_least(a.groups, 256);
@@ -492,13 +493,13 @@ extern "C" int uncl_dropout(const void* x, long long ldx, const void* res, long 
 }
 
 extern "C" int uncl_rmsnorm(const uncl_rmsnorm_desc* d, void* stream) {
-  if (!d || !dtype_ok(d->dtype) || d->rows < 0 || d->cols < 0) return UNCL_ERR_ARG;
+  if (!d || !dtype_ok(d->dtype) || !extent_ok(d->rows, d->cols)) return UNCL_ERR_ARG;
   if (d->rows == 0 || d->cols == 0) return UNCL_OK;
   const int fmt = d->y_fmt;
   if (fmt != UNCL_Q8_NONE && fmt != UNCL_E4M3 && fmt != UNCL_E5M2) return UNCL_ERR_ARG;
   if (!d->x || !d->y || !(d->eps > 0.f) || d->ldx < d->cols || d->ldy < d->cols || (d->res && d->ldr < d->cols) || (d->h && d->ldh < d->cols))
     return UNCL_ERR_ARG;
-  if (!drop_ok(d->p, d->span, d->rows, d->cols) || (fmt != UNCL_Q8_NONE && !d->y_scale)) return UNCL_ERR_ARG;
+  if (!drop_ok(d->p, d->span) || (fmt != UNCL_Q8_NONE && !d->y_scale)) return UNCL_ERR_ARG;
   NormArgs a{};
   a.x = d->x; a.res = d->res; a.w = d->weight; a.h = d->h; a.y = d->y; a.rstd = d->rstd; a.scale = d->y_scale;
   a.rows = d->rows; a.ldx = d->ldx; a.ldr = d->ldr; a.ldh = d->ldh; a.ldy = d->ldy; a.ss_row = d->scale_row; a.ss_blk = d->scale_block;
@@ -519,14 +520,14 @@ extern "C" size_t uncl_rmsnorm_backward_workspace_bytes(long long rows, int cols
 }
 
 extern "C" int uncl_rmsnorm_backward(const uncl_rmsnorm_bwd_desc* d, void* workspace, void* stream) {
-  if (!d || !dtype_ok(d->dtype) || d->rows < 0 || d->cols < 0) return UNCL_ERR_ARG;
+  if (!d || !dtype_ok(d->dtype) || !extent_ok(d->rows, d->cols)) return UNCL_ERR_ARG;
   if (d->cols == 0) return UNCL_OK;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (d->rows == 0) {
     return d->g_w ? ro_fold_rows(nullptr, 0, d->cols, d->g_w, s) : UNCL_OK;
   }
   if (!d->h || !d->rstd || d->ldh < d->cols || (d->gy && d->ldgy < d->cols) || (d->gh && d->ldgh < d->cols) ||
-      (d->g_res && d->ldgr < d->cols) || (d->g_x && d->ldgx < d->cols) || (d->g_w && !workspace) || !drop_ok(d->p, d->span, d->rows, d->cols))
+      (d->g_res && d->ldgr < d->cols) || (d->g_x && d->ldgx < d->cols) || (d->g_w && !workspace) || !drop_ok(d->p, d->span))
     return UNCL_ERR_ARG;
   NormBackArgs a{};
   a.gy = d->gy; a.gh = d->gh; a.h = d->h; a.w = d->weight; a.rstd = d->rstd; a.g_res = d->g_res; a.g_x = d->g_x;
