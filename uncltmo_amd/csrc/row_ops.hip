@@ -400,14 +400,17 @@ int grid_of(long long rows, int per, int most) {
   return (int)(b < most ? b : most);
 }
 
-// workgroups of the backward pass, a function of the shape alone (the workspace holds a row of partial sums for each): at least eight
-// rows a slot where the weight's gradient is wanted, at most 1024
+// workgroups of the backward pass, a function of the shape alone (the workspace holds a row of partial sums for each): as many as there is
+// work for up to 1024, but over 256 at least eight rows each, so that the partial sums stay under a sixteenth of what is read and written
 int back_blocks(long long rows, int cols) {
   int lanes = 256, ch = 0;
   const bool fits = row_shape(cols, lanes, ch);
   const int per = fits ? 256 / lanes : 1;
   long long b = (rows + per - 1) / per;
-  if (b > 256) { b = (b + 7) / 8; if (b < 256) b = 256; }
+  if (b > 256) {
+    const long long most = rows / 8 > 256 ? rows / 8 : 256;
+    b = b < most ? b : most;
+  }
   return (int)(b > 1024 ? 1024 : b);
 }
 
