@@ -32,9 +32,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const QuantArgs a) {
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
     if (n > 0) ro_load8(reinterpret_cast<const T*>(a.x) + row * a.ldx + col, n, v);
     bool odd;
-    unsigned m = ro_size8(v, odd);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = ro_max(m, (unsigned)__shfl_xor((int)m, o, 64));
+    const unsigned m = ro_max_lanes<16>(ro_size8(v, odd));
     const float s = ro_scale_of<FMT>(m), inv = 1.f / s;
     if (n <= 0) continue;
     ro_store8q(a.q + row * a.ldq + col, n, ro_pack8<FMT>(v, inv, odd));
@@ -147,7 +145,7 @@ __global__ __launch_bounds__(256, 2) void quant_tile_kernel(const QuantArgs a, c
     }
     __syncthreads();
   }
-  float inv = 1.f, inv_col[8];
+  float inv[8], inv_col[8];
   if constexpr (TILE) {
     unsigned m = Eight<T>::fp32_bits(all);
 #pragma unroll
@@ -155,13 +153,13 @@ __global__ __launch_bounds__(256, 2) void quant_tile_kernel(const QuantArgs a, c
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     const float s = ro_scale_of<FMT>(ro_max(ro_max(red[0], red[1]), ro_max(red[2], red[3])));
-    inv = 1.f / s;
+    const float t = 1.f / s;
     if (threadIdx.x == 0) {
       if (WAYS & 1) a.scale[blockIdx.y * a.ss_row + blockIdx.x * a.ss_blk] = s;
       if (WAYS & 2) at.scale[blockIdx.x * at.ss_row + blockIdx.y * at.ss_blk] = s;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) inv_col[j] = inv;
+    for (int j = 0; j < 8; ++j) inv[j] = inv_col[j] = t;
   } else if constexpr ((WAYS & 2) != 0) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) red[ty * 128 + tx * 8 + j] = Eight<T>::fp32_bits(by_col[j]);
@@ -178,6 +176,13 @@ __global__ __launch_bounds__(256, 2) void quant_tile_kernel(const QuantArgs a, c
 #pragma unroll
     for (int j = 0; j < 8; ++j) inv_col[j] = __builtin_bit_cast(float, red[tx * 8 + j]);
   }
+  if constexpr (!TILE && (WAYS & 1) != 0)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float s = ro_scale_of<FMT>(ro_max_lanes<16>(Eight<T>::fp32_bits(by_row[i])));
+      inv[i] = 1.f / s;
+      if (tx == 0 && row0 + ty * 8 + i < a.rows) a.scale[(row0 + ty * 8 + i) * a.ss_row + blockIdx.x * a.ss_blk] = s;
+    }
   if constexpr ((WAYS & 2) != 0) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -194,18 +199,10 @@ __global__ __launch_bounds__(256, 2) void quant_tile_kernel(const QuantArgs a, c
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const long long row = row0 + ty * 8 + i;
-      if constexpr (!TILE) {
-        unsigned m = Eight<T>::fp32_bits(by_row[i]);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = ro_max(m, (unsigned)__shfl_xor((int)m, o, 64));
-        const float s = ro_scale_of<FMT>(m);
-        inv = 1.f / s;
-        if (tx == 0 && row < a.rows) a.scale[row * a.ss_row + blockIdx.x * a.ss_blk] = s;
-      }
       float f[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = v[i].value(j);
-      if (row < a.rows && col < a.cols) ro_store8q(a.q + row * a.ldq + col, a.cols - col, ro_pack8<FMT>(f, inv, odd));
+      if (row < a.rows && col < a.cols) ro_store8q(a.q + row * a.ldq + col, a.cols - col, ro_pack8<FMT>(f, inv[i], odd));
     }
   }
   if constexpr ((WAYS & 2) != 0) {
@@ -267,25 +264,27 @@ struct LinearPlan {                      // the operands' places in one buffer, 
   size_t xq, xs, wq, ws, xt, xts, wt, wts, gq, gs, gt, gts, sums, split_y, split_gx, split_gw, end;
 };
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
-long long pitch16(long long v) { return (v + 15) & ~15ll; }
+// rows of operands begin on lines of memory: a block of 128 across two of them is two requests for the product and half-written lines here
+// (4099 rows of 2048 transposed: pitch 4112 or 4224)
+long long pitch128(long long v) { return (v + 127) & ~127ll; }
 long long blocks128(long long v) { return (v + 127) >> 7; }
 
 // what the backward pass needs from the forward one: x and w transposed
 size_t plan_saved(long long M, int N, int K, bool x, bool w, LinearPlan& p) {
   size_t at = 0;
   auto put = [&](size_t& f, size_t bytes, bool want) { f = at; at += want ? up256(bytes) : 0; };
-  put(p.xt, (size_t)K * pitch16(M), x);
+  put(p.xt, (size_t)K * pitch128(M), x);
   put(p.xts, (size_t)blocks128(M) * K * 4, x);
-  put(p.wt, (size_t)K * pitch16(N), w);
+  put(p.wt, (size_t)K * pitch128(N), w);
   put(p.wts, (size_t)blocks128(K) * blocks128(N) * 4, w);
   return at;
 }
 size_t plan_forward(long long M, int N, int K, LinearPlan& p) {
   size_t at = 0;
   auto put = [&](size_t& f, size_t bytes) { f = at; at += up256(bytes); };
-  put(p.xq, (size_t)M * pitch16(K));
+  put(p.xq, (size_t)M * pitch128(K));
   put(p.xs, (size_t)blocks128(K) * M * 4);
-  put(p.wq, (size_t)N * pitch16(K));
+  put(p.wq, (size_t)N * pitch128(K));
   put(p.ws, (size_t)blocks128(N) * blocks128(K) * 4);
   put(p.split_y, mm_split_bytes((int)M, N, K));
   return at;
@@ -293,9 +292,9 @@ size_t plan_forward(long long M, int N, int K, LinearPlan& p) {
 size_t plan_backward(long long M, int N, int K, LinearPlan& p) {
   size_t at = 0;
   auto put = [&](size_t& f, size_t bytes) { f = at; at += up256(bytes); };
-  put(p.gq, (size_t)M * pitch16(N));
+  put(p.gq, (size_t)M * pitch128(N));
   put(p.gs, (size_t)blocks128(N) * M * 4);
-  put(p.gt, (size_t)N * pitch16(M));
+  put(p.gt, (size_t)N * pitch128(M));
   put(p.gts, (size_t)blocks128(M) * N * 4);
   put(p.sums, (size_t)blocks128(M) * N * 4);
   put(p.split_gx, mm_split_bytes((int)M, K, N));
@@ -361,14 +360,14 @@ extern "C" int uncl_linear8_forward(const uncl_linear8_desc* d, void* saved, voi
   plan_saved(M, N, K, d->for_w, d->for_x, p);
   plan_forward(M, N, K, p);
   char *ws = reinterpret_cast<char*>(workspace), *sv = reinterpret_cast<char*>(saved);
-  const QuantArgs x = quant_args(d->x, M, K, d->ldx, ws + p.xq, pitch16(K), ws + p.xs, 1, M);
-  const QuantArgs xt = quant_args(d->x, M, K, d->ldx, sv + p.xt, pitch16(M), sv + p.xts, 1, K);
-  const QuantArgs w = quant_args(d->w, N, K, d->ldw, ws + p.wq, pitch16(K), ws + p.ws, blocks128(K), 1);
-  const QuantArgs wt = quant_args(d->w, N, K, d->ldw, sv + p.wt, pitch16(N), sv + p.wts, blocks128(N), 1);
+  const QuantArgs x = quant_args(d->x, M, K, d->ldx, ws + p.xq, pitch128(K), ws + p.xs, 1, M);
+  const QuantArgs xt = quant_args(d->x, M, K, d->ldx, sv + p.xt, pitch128(M), sv + p.xts, 1, K);
+  const QuantArgs w = quant_args(d->w, N, K, d->ldw, ws + p.wq, pitch128(K), ws + p.ws, blocks128(K), 1);
+  const QuantArgs wt = quant_args(d->w, N, K, d->ldw, sv + p.wt, pitch128(N), sv + p.wts, blocks128(N), 1);
   int rc = LIN_BY_TYPE(d->dtype, quant_x, x, xt, d->for_w != 0, s);
   if (rc == UNCL_OK) rc = LIN_BY_TYPE(d->w_dtype, quant_w, w, wt, d->for_x != 0, s);
   if (rc != UNCL_OK) return rc;
-  MmArgs m = product(ws + p.xq, pitch16(K), ws + p.xs, ws + p.wq, pitch16(K), ws + p.ws, blocks128(K), 1, M, N, K, d->y, d->ldy, d->dtype);
+  MmArgs m = product(ws + p.xq, pitch128(K), ws + p.xs, ws + p.wq, pitch128(K), ws + p.ws, blocks128(K), 1, M, N, K, d->y, d->ldy, d->dtype);
   m.bias = d->bias;
   return mm_run(m, UNCL_E4M3, true, ws + p.split_y, s);
 }
@@ -385,15 +384,15 @@ extern "C" int uncl_linear8_backward(const uncl_linear8_desc* d, const void* sav
   plan_backward(M, N, K, p);
   char* ws = reinterpret_cast<char*>(workspace);
   const char* sv = reinterpret_cast<const char*>(saved);
-  const QuantArgs g = quant_args(d->gy, M, N, d->ldgy, ws + p.gq, pitch16(N), ws + p.gs, 1, M);
-  const QuantArgs gt = quant_args(d->gy, M, N, d->ldgy, ws + p.gt, pitch16(M), ws + p.gts, 1, N);
+  const QuantArgs g = quant_args(d->gy, M, N, d->ldgy, ws + p.gq, pitch128(N), ws + p.gs, 1, M);
+  const QuantArgs gt = quant_args(d->gy, M, N, d->ldgy, ws + p.gt, pitch128(M), ws + p.gts, 1, N);
   float* sums = reinterpret_cast<float*>(ws + p.sums);
   int rc = LIN_BY_TYPE(d->dtype, quant_g, g, gt, d->grad_fmt, d->gw != nullptr, sums, s);
   if (rc == UNCL_OK && d->gx)
-    rc = mm_run(product(ws + p.gq, pitch16(N), ws + p.gs, sv + p.wt, pitch16(N), sv + p.wts, blocks128(N), 1, M, K, N, d->gx, d->ldgx, d->dtype), d->grad_fmt,
+    rc = mm_run(product(ws + p.gq, pitch128(N), ws + p.gs, sv + p.wt, pitch128(N), sv + p.wts, blocks128(N), 1, M, K, N, d->gx, d->ldgx, d->dtype), d->grad_fmt,
                 true, ws + p.split_gx, s);
   if (rc == UNCL_OK && d->gw)
-    rc = mm_run(product(ws + p.gt, pitch16(M), ws + p.gts, sv + p.xt, pitch16(M), sv + p.xts, 1, K, N, K, M, d->gw, d->ldgw, d->w_dtype), d->grad_fmt, false,
+    rc = mm_run(product(ws + p.gt, pitch128(M), ws + p.gts, sv + p.xt, pitch128(M), sv + p.xts, 1, K, N, K, M, d->gw, d->ldgw, d->w_dtype), d->grad_fmt, false,
                 ws + p.split_gw, s);
   if (rc == UNCL_OK && d->gb) rc = ro_fold_rows(sums, (int)blocks128(M), N, d->gb, s);
   return rc;

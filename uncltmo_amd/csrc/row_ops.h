@@ -113,6 +113,20 @@ __device__ __forceinline__ unsigned ro_size(float v) {
   return ODD && u >= RO_INF_BITS ? 0u : u;
 }
 __device__ __forceinline__ unsigned ro_max(unsigned a, unsigned b) { return a > b ? a : b; }
+// maximum over LANES (1 .. 16) neighbouring lanes; every one of them gets it.  Quads, mirrored halves and rows of sixteen by data-parallel
+// moves: no trip through LDS
+template <int CTRL>
+__device__ __forceinline__ unsigned ro_moved(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int LANES>
+__device__ __forceinline__ unsigned ro_max_lanes(unsigned m) {
+  if constexpr (LANES >= 2) m = ro_max(m, ro_moved<0xB1>(m));      // lanes 1 0 3 2 of each four
+  if constexpr (LANES >= 4) m = ro_max(m, ro_moved<0x4E>(m));      // lanes 2 3 0 1
+  if constexpr (LANES >= 8) m = ro_max(m, ro_moved<0x141>(m));     // eight lanes mirrored: the other four
+  if constexpr (LANES >= 16) m = ro_max(m, ro_moved<0x140>(m));    // sixteen lanes mirrored: the other eight
+  return m;
+}
 // largest finite size of eight; odd: whether one of them is not finite
 __device__ __forceinline__ unsigned ro_size8(const float* v, bool& odd) {
   unsigned m = 0;

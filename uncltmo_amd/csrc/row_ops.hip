@@ -99,9 +99,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a) {
         if (n > 0) ro_store8(reinterpret_cast<T*>(a.y) + row * a.ldy + col, n, y);
       } else {
         bool odd;
-        unsigned m = ro_size8(y, odd);
-#pragma unroll
-        for (int o = (LANES < 16 ? LANES : 16) / 2; o > 0; o >>= 1) m = ro_max(m, (unsigned)__shfl_xor((int)m, o, 64));
+        const unsigned m = ro_max_lanes<(LANES < 16 ? LANES : 16)>(ro_size8(y, odd));
         const float s = ro_scale_of<FMT>(m), inv = 1.f / s;
         if (n > 0) {
           ro_store8q(reinterpret_cast<unsigned char*>(a.y) + row * a.ldy + col, n, ro_pack8<FMT>(y, inv, odd));
@@ -160,9 +158,7 @@ __global__ __launch_bounds__(256) void norm_long_kernel(const NormArgs a) {
         if (n > 0) ro_store8(reinterpret_cast<T*>(a.y) + row * a.ldy + col, n, v);
       } else {
         bool odd;
-        unsigned m = ro_size8(v, odd);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = ro_max(m, (unsigned)__shfl_xor((int)m, o, 64));
+        const unsigned m = ro_max_lanes<16>(ro_size8(v, odd));
         const float s = ro_scale_of<FMT>(m), inv = 1.f / s;
         if (n > 0) {
           ro_store8q(reinterpret_cast<unsigned char*>(a.y) + row * a.ldy + col, n, ro_pack8<FMT>(v, inv, odd));

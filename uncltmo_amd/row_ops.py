@@ -314,8 +314,8 @@ def _no_grad(what, *ts):
 
 
 def _empty8(rows, cols, fmt, block, dev):
-    """rows on 16-byte borders; row scales lie block by block, as the product reads them"""
-    pitch, kb = (cols + 15) & ~15, (cols + 127) // BLOCK
+    """rows on lines of memory (16-byte borders if they are shorter than one); row scales lie block by block, as the product reads them"""
+    pitch, kb = (cols + 127) & ~127 if cols >= BLOCK else (cols + 15) & ~15, (cols + 127) // BLOCK
     data = torch.empty(rows, pitch, dtype=_F8[fmt], device=dev)
     if pitch != cols:
         data = data[:, :cols]
