@@ -304,7 +304,7 @@ def test_norm_into_8_bits(dtype, cols, fmt):
 
 
 # ---- product -----------------------------------------------------------------------------------------------------------------------------
-def operand(rows, cols, block, fmt="e4m3", seed=0, garbage=True):
+def operand(rows, cols, block, fmt="e4m3", seed=0):
     """a quantised matrix whose bytes behind a row's end are NaN"""
     data, scale = R.quantize(rnd(rows, cols, seed=seed) * torch.exp2(torch.arange(cols) % 5 - 2.0), block, fmt)
     room = torch.full((rows, -(-cols // 16) * 16 + 16), 0x7F, dtype=torch.uint8, device="cuda")
@@ -420,6 +420,10 @@ def test_product_layouts():
     assert torch.equal(acc, want + 1)
     r = rnd(n, m).cuda().t()                                                            # a residual with columns apart
     assert torch.equal(row_ops.matmul8(a, b, out_dtype=torch.float32, residual=r), want + r)
+    run = torch.arange((m + 1) * n, device="cuda", dtype=torch.float32).view(m + 1, n) % 64    # a residual one row above the result
+    above = run[:-1].clone()
+    row_ops.matmul8(a, b, out_dtype=torch.float32, residual=run[:-1], out=run[1:])
+    assert torch.equal(run[1:], want + above)
     e = row_ops.matmul8(row_ops.Quant8(a.data[:0], a.scale[:0], "row"), b)
     assert e.shape == (0, n)
 
@@ -443,6 +447,7 @@ def test_product_refusals():
                        (lambda: row_ops.quantize8(torch.zeros(4, 4, device="cuda", requires_grad=True)), RuntimeError),
                        (lambda: row_ops.dropout(torch.zeros(4, 4, device="cuda"), 1.5, 1), ValueError),
                        (lambda: row_ops.dropout(torch.zeros(4, 4, device="cuda"), 0.5, 1, span=0), ValueError),
+                       (lambda: row_ops.dropout(torch.zeros(4, 4, device="cuda"), 0.5, 1, span=2 ** 64 + 1), ValueError),
                        (lambda: row_ops.dropout(torch.zeros(4, 4, device="cuda"), 0.5, 1.5), TypeError),
                        (lambda: row_ops.dropout(torch.zeros(4, 4, device="cuda"), 0.5, torch.zeros(2, dtype=torch.int64)), _hip.HipError),
                        (lambda: row_ops.dropout(torch.zeros((), device="cuda"), 0.5, 1), ValueError),
@@ -451,6 +456,7 @@ def test_product_refusals():
                        (lambda: row_ops.rms_norm(torch.zeros(4, 4, device="cuda"), torch.ones(5, device="cuda")), ValueError),
                        (lambda: row_ops.rms_norm(torch.zeros(4, 4, device="cuda"), eps=0.0), ValueError),
                        (lambda: row_ops.linear8(torch.zeros(4, 4, device="cuda"), torch.zeros(5, 3, device="cuda")), ValueError),
+                       (lambda: row_ops.linear8(torch.zeros(1, 1, device="cuda").expand(2 ** 22 + 1, 1), torch.zeros(1, 1, device="cuda")), ValueError),
                        (lambda: row_ops.linear8(torch.zeros(4, 4, device="cuda"), torch.zeros(5, 4, device="cuda"), grad_fmt="fp8"), ValueError)):
         with pytest.raises(kind):
             call()

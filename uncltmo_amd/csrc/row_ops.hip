@@ -9,6 +9,11 @@
 // All of them are bound by HBM: each input is read once, each output written once, the row lives in registers between the two passes
 // over it.  A row is held by LANES threads, eight channels each per chunk, CH chunks: narrow maps (32 channels: 4 lanes) put sixteen rows
 // into a wave, so that every access of a wave is 1 KB of consecutive memory whatever the width.
+//
+// Measured, bf16 (a copy of 1 GiB runs at 5.05 TB/s on the same card): dropout of 16 x 252 x 252 x 32 25.6 us = 5.1 TB/s (a
+// Philox evaluation of ten rounds for each eight elements hides behind the loads); addition and norm of 8 x 252 x 252 x 32 28.7 us and the
+// backward pass 29.9 + 4.1 us (fold of the weight gradient) = 4.4 TB/s; into 8 bits 28800 x 256 11.7 us = 4.5 TB/s; a single row 3.4 us,
+// of which the launch is most.
 #include "row_ops.h"
 
 namespace {

@@ -99,8 +99,8 @@ def _seed_args(p, seed, offset, span, dev):
     p = float(p)
     if not 0.0 <= p <= 1.0:
         raise ValueError("uncltmo_amd: the dropout probability must be in [0, 1], got %r" % p)
-    if not isinstance(span, int) or span < 1:
-        raise ValueError("uncltmo_amd: span (rows that share their flags) must be a positive integer, got %r" % (span,))
+    if not isinstance(span, int) or not 1 <= span < 1 << 63:
+        raise ValueError("uncltmo_amd: span (rows that share their flags) must be a positive integer of 64 bits, got %r" % (span,))
     if not isinstance(offset, int):
         raise TypeError("uncltmo_amd: offset must be an integer, got %s" % type(offset).__name__)
     if isinstance(seed, torch.Tensor):
@@ -429,6 +429,9 @@ def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16
         return out
     if residual is not None:
         residual, d.ldr = _rows(residual)
+        if residual.data_ptr() != out.data_ptr() or d.ldr != ldo:        # rows of the one that are other rows of the other would be read too late
+            if residual.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
+                residual, d.ldr = residual.clone(memory_format=torch.contiguous_format), n
         d.res = residual.data_ptr()
     tile = b.block == "tile"
     (ad, lda), (bd, ldb), (sa, sas), (sb, sbs) = _operand(ad), _operand(bd), _scale(a.scale), _scale(b.scale, 1 << 20 if tile else 1)
@@ -504,12 +507,15 @@ def linear8(x, weight, bias=None, grad_fmt="e5m2"):
     """x weight^T + bias with all three products of a training step in 8 bits: x and weight are quantised to e4m3 (rows / tiles of 128), the
     gradient of the output to grad_fmt by rows -- along its columns for x's gradient, along its rows, like x, for weight's.  weight (N, K)
     fp32, bf16 or fp16; bias fp32 (N).  The result and x's gradient have x's type, weight's gradient weight's (summed in fp32).  The rounding
-    of the operands is not differentiated (straight through).  What the backward pass needs of x and weight is kept in 8 bits."""
+    of the operands is not differentiated (straight through).  What the backward pass needs of x and weight is kept in 8 bits.  Up to 2^22
+    rows, channels and results (each is a common axis of one of the products)."""
     _need(x, "x", _DTYPES)
     rows, k = _extent(x)
     _need(weight, "weight", _DTYPES, None, x.device)
     if weight.dim() != 2 or weight.shape[1] != k or k == 0 or weight.shape[0] == 0:
         raise ValueError("uncltmo_amd: weight must be (N, %d) with N > 0 and channels to sum over, got %s" % (k, tuple(weight.shape)))
+    if max(rows, k, weight.shape[0]) > 1 << 22:
+        raise ValueError("uncltmo_amd: linear8 takes up to 2^22 rows, channels and results, got %d, %d and %d" % (rows, k, weight.shape[0]))
     if bias is not None:
         _need(bias, "bias", (torch.float32,), (weight.shape[0],), x.device)
     _fmt(grad_fmt)
