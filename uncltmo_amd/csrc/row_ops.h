@@ -45,6 +45,23 @@ __device__ __forceinline__ void ro_store8(T* p, int n, const float* f) {
   }
 }
 
+// eight whole elements as they lie, for loads that are not waited for at once
+template <typename T>
+struct RoRaw8 {
+  f32x4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(v, p, 8 * sizeof(T)); }
+  __device__ __forceinline__ void get(float* f) const {
+    if constexpr (sizeof(T) == 2) {
+      typename Elem<T>::vec x;
+      __builtin_memcpy(&x, v, 16);
+      Elem<T>::unpack(x, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { f[i] = v[0][i]; f[4 + i] = v[1][i]; }
+    }
+  }
+};
+
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011): counter (group, stream), key = seed.
 __device__ __forceinline__ void ro_philox(unsigned long long group, unsigned long long stream, unsigned long long seed, unsigned* w) {
   unsigned c0 = (unsigned)group, c1 = (unsigned)(group >> 32), c2 = (unsigned)stream, c3 = (unsigned)(stream >> 32);
