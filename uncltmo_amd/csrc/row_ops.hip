@@ -10,10 +10,10 @@
 // over it.  A row is held by LANES threads, eight channels each per chunk, CH chunks: narrow maps (32 channels: 4 lanes) put sixteen rows
 // into a wave, so that every access of a wave is 1 KB of consecutive memory whatever the width.
 //
-// Measured, bf16 (a copy of 1 GiB runs at 5.05 TB/s on the same card): dropout of 16 x 252 x 252 x 32 25.6 us = 5.1 TB/s (a
-// Philox evaluation of ten rounds for each eight elements hides behind the loads); addition and norm of 8 x 252 x 252 x 32 28.7 us and the
-// backward pass 29.9 + 4.1 us (fold of the weight gradient) = 4.4 TB/s; into 8 bits 28800 x 256 11.7 us = 4.5 TB/s; a single row 3.4 us,
-// of which the launch is most.
+// Measured, bf16 (a copy of 1 GiB runs at 5.05 TB/s on the same card): dropout of 16 x 252 x 252 x 32 25.6 us = 5.1 TB/s (a Philox
+// evaluation of ten rounds for each eight elements hides behind the loads); addition and norm of 8 x 252 x 252 x 32 28.4 us = 4.6 TB/s,
+// the backward pass 24.9 us = 5.2 TB/s and 4.1 us for the weight gradient's fold; into 8 bits 28800 x 256 11.5 us = 4.6 TB/s; a single row
+// 3.4 us, of which the launch is most.
 #include "row_ops.h"
 
 namespace {
@@ -402,7 +402,8 @@ int grid_of(long long rows, int per, int most) {
 }
 
 // workgroups of the backward pass, a function of the shape alone (the workspace holds a row of partial sums for each): as many as there is
-// work for up to 1024 (20000 x 4096 bf16: 107 us; 512 156, 2048 116), but over 256 at least eight rows each, so that the partial sums stay under a sixteenth of what is read and written
+// work for up to 1024 (20000 x 4096 bf16: 107 us; 512 156, 2048 116), but over 256 at least eight rows each, so that the partial sums stay
+// under a sixteenth of what is read and written
 int back_blocks(long long rows, int cols) {
   int lanes = 256, ch = 0;
   const bool fits = row_shape(cols, lanes, ch);
