@@ -428,6 +428,21 @@ def test_product_layouts():
     assert e.shape == (0, n)
 
 
+@pytest.mark.parametrize("m,k", [(3, 128), (100, 256), (70, 4096)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_product_activations_of_what_is_not_finite(m, k, dtype):
+    _, a = operand(m, k, "row")
+    _, b = operand(5, k, "tile")
+    inf, nan = float("inf"), float("nan")
+    bias = torch.tensor([inf, -inf, nan, -1e30, 1e30 if dtype != torch.float16 else 6e4], device="cuda")
+    for act, want in (("none", [inf, -inf, nan]), ("relu", [inf, 0.0, nan]), ("lrelu", [inf, -inf, nan]), ("gelu", [inf, 0.0, nan]),
+                      ("sigmoid", [1.0, 0.0, nan]), ("tanh", [1.0, -1.0, nan]), ("msig", [1.0, 0.0, nan])):
+        out = row_ops.matmul8(a, b, bias=bias, act=act, out_dtype=dtype).float()
+        assert torch.equal(out[:, :3].nan_to_num(7.0, 8.0, -8.0), torch.tensor(want, device="cuda").nan_to_num(7.0, 8.0, -8.0).expand(m, 3)), act
+        if act in ("relu", "gelu"):
+            assert (out[:, 3] == 0).all() and torch.isfinite(out[:, 4]).all()
+
+
 def test_product_refusals():
     _, a = operand(8, 64, "row")
     _, b = operand(8, 64, "tile")

@@ -74,9 +74,10 @@ __device__ __forceinline__ void mm_block(const Wide (&b)[TN], const Wide& a, f32
 }
 
 // x Phi(x) = max(x, 0) - |x| (1 - Phi(|x|)), the tail by Abramowitz and Stegun 7.1.26 (erf off by at most 1.5e-7): the library's erff took
-// half of a short product's time
+// half of a short product's time.  |x| stops at 64, where the tail is 0 long since, so that infinity times it is not NaN: infinity stays,
+// minus infinity becomes 0.
 __device__ __forceinline__ float mm_gelu(float x) {
-  const float a = __builtin_fabsf(x);
+  const float a = fminf(__builtin_fabsf(x), 64.f);
   const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, a, 1.f));
   float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
   q = fmaf(t, q, 0.5f * 1.421413741f);
@@ -96,7 +97,7 @@ __device__ __forceinline__ void mm_act(float* v, int act) {
     for (int i = 0; i < E; ++i) v[i] = mm_gelu(v[i]);
   } else if (act == UNCL_ACT_RELU) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = v[i] > 0.f ? v[i] : 0.f;
+    for (int i = 0; i < E; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];             // (NaN stays)
   } else if (act != UNCL_ACT_NONE) {
 #pragma unroll
     for (int i = 0; i < E; ++i) v[i] = mm_act_rare(v[i], act);
