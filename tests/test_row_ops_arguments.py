@@ -1,0 +1,59 @@
+"""What the Python entry points of the operators on rows of channels (uncltmo_amd.row_ops) decide before a launch, without a GPU: the device
+check and the launch are replaced, so that sizes can be those of tensors that no memory holds."""
+import pytest
+import torch
+
+from uncltmo_amd import row_ops
+
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """entry points called, in place of launches"""
+    seen = []
+    monkeypatch.setattr(row_ops, "_need", lambda t, what, dtypes, shape=None, dev=None: t)
+    monkeypatch.setattr(row_ops, "_call", lambda dev, what, fn, *args: seen.append(what))
+    return seen
+
+
+def meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+def q8(rows, cols, block, pitch=None):
+    """a matrix in 8 bits without memory"""
+    pitch = pitch or (cols + 15) & ~15
+    data = meta(rows, pitch, dtype=E4M3)[:, :cols]
+    return row_ops.Quant8(data, meta(rows if block == "row" else (rows + 127) // 128, (cols + 127) // 128, dtype=torch.float32), block)
+
+
+# sizes that a 32-bit field would keep the low bits of, and the first ones over the limits
+WIDE = [(2 ** 32,), (2 ** 32 + 8,), (3, 2 ** 32 + 8), (2 ** 30 + 1,), (1, 2, 2 ** 31)]
+
+
+@pytest.mark.parametrize("shape", WIDE + [(2 ** 32 + 1, 4), (2 ** 17, 2 ** 16, 1)], ids=str)
+def test_rows_and_channels_over_the_limits_are_refused(calls, shape):
+    x = meta(*shape)
+    for call in (lambda: row_ops.dropout(x, 0.5, 1), lambda: row_ops.rms_norm(x), lambda: row_ops.add_rms_norm(x, x, p=0.1),
+                 lambda: row_ops.rms_norm_quant8(x), lambda: row_ops.quantize8(x), lambda: row_ops.quantize8(x, "tile"),
+                 lambda: row_ops.quantize8(x, transpose=True), lambda: row_ops.linear8(x, meta(8, shape[-1]))):
+        with pytest.raises(ValueError):
+            call()
+    assert not calls
+
+
+def test_rows_and_channels_at_the_limits_are_taken(calls):
+    for x in (meta(2 ** 30), meta(2 ** 32, 1)):
+        row_ops.dropout(x, 0.5, 1)
+        row_ops.rms_norm(x)
+        row_ops.quantize8(x)
+    assert calls == ["uncl_dropout", "uncl_rmsnorm", "uncl_quant8"] * 2
+
+
+@pytest.mark.parametrize("m,n,k", [(2 ** 32 + 5, 8, 16), (2 ** 32, 8, 16), (8, 2 ** 32 + 8, 16), (2 ** 30 + 1, 8, 16), (8, 2 ** 30 + 1, 16), (8, 8, 2 ** 32 + 128),
+                                   (8, 8, 2 ** 22 + 1)])
+def test_products_over_the_limits_are_refused(calls, m, n, k):
+    with pytest.raises(ValueError):
+        row_ops.matmul8(q8(m, k, "row"), q8(n, k, "tile"))
+    assert not calls

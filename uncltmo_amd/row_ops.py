@@ -87,11 +87,14 @@ def _rows(t):
 
 
 def _extent(x):
-    """(rows, channels)"""
+    """(rows, channels), within what the entry points take: they hold channels in 32 bits, and ctypes would cut a larger number off unasked"""
     if x.dim() == 0:
         raise ValueError("uncltmo_amd: a tensor of rows needs an axis of channels")
     s = x.shape
-    return (s[0] if len(s) == 2 else s[:-1].numel()), s[-1]
+    rows, cols = s[0] if len(s) == 2 else s[:-1].numel(), s[-1]
+    if rows > 1 << 32 or cols > 1 << 30:
+        raise ValueError("uncltmo_amd: up to 2^32 rows of up to 2^30 channels, got %d of %d" % (rows, cols))
+    return rows, cols
 
 
 def _seed_args(p, seed, offset, span, dev):
@@ -407,6 +410,8 @@ def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16
         raise ValueError("uncltmo_amd: a is (M, K) = %s on %s, b (N, K) = %s on %s" % ((m, k), dev, (n, kb), bd.device))
     if k == 0:
         raise ValueError("uncltmo_amd: matmul8 needs a common axis of at least one element")
+    if max(m, n) > 1 << 30 or k > 1 << 22:
+        raise ValueError("uncltmo_amd: matmul8 takes up to 2^30 rows and results and a common axis of up to 2^22, got %d, %d and %d" % (m, n, k))
     if act not in _ACT:
         raise ValueError("uncltmo_amd: unknown activation %r" % (act,))
     if out_dtype not in _CODE:
