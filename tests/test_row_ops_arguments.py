@@ -57,3 +57,20 @@ def test_products_over_the_limits_are_refused(calls, m, n, k):
     with pytest.raises(ValueError):
         row_ops.matmul8(q8(m, k, "row"), q8(n, k, "tile"))
     assert not calls
+
+
+def test_forward_mode_derivatives_are_refused(calls):
+    """a dual tensor needs no requires_grad; its tangent must not get lost"""
+    x, other, w = torch.ones(4, 16), torch.zeros(4, 16), torch.ones(16)
+    quants = row_ops.Quant8(x.to(E4M3), torch.ones(4, 1), "row"), row_ops.Quant8(x.to(E4M3), torch.ones(1, 1), "tile")
+    with torch.autograd.forward_ad.dual_level():
+        d, dw = (torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w))
+        for call in (lambda: row_ops.dropout(d, 0.5, 1), lambda: row_ops.dropout(x, 0.5, 1, residual=d), lambda: row_ops.rms_norm(d), lambda: row_ops.rms_norm(x, dw),
+                     lambda: row_ops.add_rms_norm(x, d), lambda: row_ops.rms_norm_quant8(d), lambda: row_ops.quantize8(d), lambda: row_ops.linear8(d, other),
+                     lambda: row_ops.linear8(x, d), lambda: row_ops.matmul8(*quants, residual=torch.autograd.forward_ad.make_dual(other[:, :4], other[:, :4]))):
+            for mode in (torch.enable_grad, torch.no_grad):              # (no_grad leaves forward mode on)
+                with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        assert not calls
+        row_ops.dropout(x, 0.5, 1)                                       # no tangent: an ordinary call
+    assert calls == ["uncl_dropout"]

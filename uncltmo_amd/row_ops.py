@@ -14,6 +14,7 @@ import ctypes as C
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _hip
@@ -269,6 +270,10 @@ def _norm_checks(x, residual, weight, eps):
 
 
 def _wants_grad(a, b=None, c=None):
+    """whether the call belongs on autograd's tape.  A dual tensor needs no requires_grad (and torch.no_grad() does not stop it): its tangent would
+    get lost without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (a, b, c)):
+        raise NotImplementedError("uncltmo_amd: the operators on rows of channels have no forward-mode derivatives")
     return torch.is_grad_enabled() and ((a is not None and a.requires_grad) or (b is not None and b.requires_grad) or (c is not None and c.requires_grad))
 
 
