@@ -74,3 +74,22 @@ def test_forward_mode_derivatives_are_refused(calls):
         assert not calls
         row_ops.dropout(x, 0.5, 1)                                       # no tangent: an ordinary call
     assert calls == ["uncl_dropout"]
+
+
+def test_product_into_a_given_tensor_is_a_change_that_autograd_sees(calls):
+    """written as torch's own in-place operations are: a backward pass that saved the tensor raises instead of reading the new numbers"""
+    a, b = row_ops.Quant8(torch.ones(4, 16).to(E4M3), torch.ones(4, 1), "row"), row_ops.Quant8(torch.ones(16, 16).to(E4M3), torch.ones(1, 1), "tile")
+    x = torch.ones(4, 16, requires_grad=True)
+    h = x * 2
+    y = h * h                                                            # saves h
+    with torch.no_grad():
+        row_ops.matmul8(a, b, residual=h.detach(), out_dtype=torch.float32, out=h.detach())
+    assert calls == ["uncl_matmul8"] and h._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        t = torch.zeros(4, 16)
+        assert row_ops.matmul8(a, b, out_dtype=torch.float32, out=t) is t
+    empty = row_ops.Quant8(a.data[:0], a.scale[:0], "row")
+    row_ops.matmul8(empty, b, out_dtype=torch.float32, out=torch.zeros(0, 16))
+    assert len(calls) == 2

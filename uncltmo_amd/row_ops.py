@@ -428,7 +428,8 @@ def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16
     if residual is not None:
         _need(residual, "residual", (out_dtype,), (m, n), dev)
     _no_grad("matmul8", bias, residual, out)
-    if out is None:
+    given = out is not None
+    if not given:
         out, ldo = torch.empty(m, n, dtype=out_dtype, device=dev), n
     else:
         _need(out, "out", (out_dtype,), (m, n), dev)
@@ -453,6 +454,8 @@ def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16
     size = lib.uncl_matmul8_workspace_bytes(m, n, k) if m > 64 else 0
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     _call(dev, "uncl_matmul8", lib.uncl_matmul8, C.byref(d), None if ws is None else ws.data_ptr())
+    if given:                                                # autograd's saved copy of it, if there is one, is no longer what was saved
+        torch.autograd.graph.increment_version(out)
     return out
 
 
