@@ -799,7 +799,8 @@ int uncl_rmsnorm_backward(const uncl_rmsnorm_bwd_desc* d, void* workspace, void*
  * x * fl(1 / scale).  amax is over the finite elements of the block; an infinity becomes the largest number, a NaN stays NaN.
  * tile = 0: blocks of 128 along the rows of q (1 x 128); tile = 1: blocks of 128 x 128.  transposed = 1: q is x's transpose (cols rows of
  * `rows` elements, blocks of 128 along x's rows).  q: bytes, rows ldq bytes apart (bytes behind a row's end are not written);
- * scale[r * scale_row + b * scale_block], r = row of q (tile: row / 128), b = block along it. */
+ * scale[r * scale_row + b * scale_block], r = row of q (tile: row / 128), b = block along it.  tile = 1 or transposed = 1: up to 65535 x 128
+ * rows. */
 int uncl_quant8(const void* x, int dtype, long long rows, int cols, long long ldx, void* q, long long ldq, int fmt, float* scale,
                 long long scale_row, long long scale_block, int tile, int transposed, void* stream);
 

@@ -93,3 +93,13 @@ def test_product_into_a_given_tensor_is_a_change_that_autograd_sees(calls):
     empty = row_ops.Quant8(a.data[:0], a.scale[:0], "row")
     row_ops.matmul8(empty, b, out_dtype=torch.float32, out=torch.zeros(0, 16))
     assert len(calls) == 2
+
+
+def test_quantised_tiles_have_a_limit_of_rows(calls):
+    most = 65535 * 128
+    for kw in (dict(block="tile"), dict(transpose=True), dict(block="tile", transpose=True)):
+        row_ops.quantize8(meta(most, 8), **kw)
+        with pytest.raises(ValueError, match="8388480"):
+            row_ops.quantize8(meta(most + 1, 8), **kw)
+    row_ops.quantize8(meta(most + 1, 8))
+    assert calls == ["uncl_quant8"] * 4

@@ -20,6 +20,7 @@ from torch.autograd.function import once_differentiable
 from . import _hip
 
 BLOCK = 128
+_TILED_ROWS = 65535 * BLOCK               # one workgroup a tile of 128 x 128, tiles of rows along the grid's second axis
 _FMT = {"e4m3": _hip.E4M3, "e5m2": _hip.E5M2}
 _F8 = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 _F8_TYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
@@ -356,13 +357,15 @@ def quantize8(x, block="row", transpose=False, fmt="e4m3"):
     """x (rows, cols) -- leading axes of a larger tensor are its rows -- in 8 bits, block by block: scale = max(amax, 2^-100) / largest number
     of the format, data = x / scale rounded to the nearest, ties to even.  block "row": 1 x 128 (activations, gradients); "tile": 128 x 128
     (weights).  transpose: the result is (cols, rows), its blocks along x's rows.  Infinities become the largest number, NaN stays NaN;
-    neither counts for the block's scale."""
+    neither counts for the block's scale.  By tiles or transposed: up to 65535 x 128 rows."""
     _need(x, "x", _DTYPES)
     code = _fmt(fmt)
     if block not in ("row", "tile"):
         raise ValueError("uncltmo_amd: block must be 'row' or 'tile', got %r" % (block,))
     _no_grad("quantize8", x)
     rows, cols = _extent(x)
+    if rows > _TILED_ROWS and (block == "tile" or transpose):
+        raise ValueError("uncltmo_amd: quantize8 by tiles or transposed takes up to %d rows, got %d" % (_TILED_ROWS, rows))
     x, ldx = _rows(x)
     q = _empty8(cols if transpose else rows, rows if transpose else cols, fmt, block, x.device)
     _call(x.device, "uncl_quant8", _hip.lib().uncl_quant8, x.data_ptr(), _CODE[x.dtype], rows, cols, ldx, q.data.data_ptr(), q.data.stride(0), code,
