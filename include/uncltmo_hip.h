@@ -836,7 +836,8 @@ int uncl_matmul8(const uncl_matmul8_desc* d, void* workspace, void* stream);
 
 /* The linear layer of a training step from three such products: y = x w^T + bias (x (M, K), w (N, K): e4m3, rows / tiles of 128),
  * gx = gy w (gy (M, N) in grad_fmt by rows, w by tiles), gw = gy^T x (both by 128s along M), gb = the columns' sums of gy.  x, gy, y, gx are
- * `dtype`, w and gw `w_dtype`, bias and gb fp32.  M, N, K to 2^22.
+ * `dtype`, w and gw `w_dtype`, bias and gb fp32.  M, N, K to 2^22.  An infinity in x, w or gy counts as NaN: every y, gx and gw that it takes
+ * part in is NaN, the others are as if it were 0 (gb is the plain sum).
  * forward: for_x / for_w = which of gx / gw will be asked for; `saved` (uncl_linear8_saved_bytes) then takes w and / or x in 8 bits,
  * transposed, which is all that the backward pass needs of them; NULL if neither.  y and bias (NULL: none) as in uncl_matmul8.
  * backward: the same for_x / for_w and `saved`; gx, gw, gb: NULL where not wanted.  workspace: uncl_linear8_workspace_bytes(.., backward).

@@ -18,6 +18,7 @@ struct QuantArgs {
   float* scale;
   long long rows, ldx, ldq, ss_row, ss_blk;
   int cols;
+  bool lost;                             // infinities become NaN, not the largest number
 };
 
 // 1 x 128 blocks along the row: sixteen lanes hold one block, a wave four
@@ -37,7 +38,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const QuantArgs a) {
     const unsigned m = ro_max_lanes<16>(ro_size8(v, odd));
     const float s = ro_scale_of<FMT>(m), inv = 1.f / s;
     if (n <= 0) continue;
-    ro_store8q(a.q + row * a.ldq + col, n, ro_pack8<FMT>(v, inv, odd));
+    ro_store8q(a.q + row * a.ldq + col, n, ro_pack8<FMT>(v, inv, odd, a.lost));
     if (lane == 0) a.scale[row * a.ss_row + kb * a.ss_blk] = s;
   }
 }
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(256, 2) void quant_tile_kernel(const QuantArgs a, c
       float f[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = v[i].value(j);
-      const u32x2 b = ro_pack8<FMT>(f, inv_col[j], odd);
+      const u32x2 b = ro_pack8<FMT>(f, inv_col[j], odd, a.lost);
       unsigned* to = reinterpret_cast<unsigned*>(&turn[(tx * 8 + j) * 132 + ty * 8]);
       to[0] = b[0];
       to[1] = b[1];
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(256, 2) void quant_tile_kernel(const QuantArgs a, c
       float f[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = v[i].value(j);
-      if (row < a.rows && col < a.cols) ro_store8q(a.q + row * a.ldq + col, a.cols - col, ro_pack8<FMT>(f, inv[i], odd));
+      if (row < a.rows && col < a.cols) ro_store8q(a.q + row * a.ldq + col, a.cols - col, ro_pack8<FMT>(f, inv[i], odd, a.lost));
     }
   }
   if constexpr ((WAYS & 2) != 0) {
@@ -247,7 +248,7 @@ extern "C" int uncl_quant8(const void* x, int dtype, long long rows, int cols, l
   if (rows == 0 || cols == 0) return UNCL_OK;
   if (!x || !q || !scale || ldx < cols || ldq < (transposed ? rows : cols)) return UNCL_ERR_ARG;
   if ((tile || transposed) && (rows + 127) / 128 > 65535) return UNCL_ERR_ARG;      // one workgroup a tile, rows along the grid's y
-  const QuantArgs a{x, reinterpret_cast<unsigned char*>(q), scale, rows, ldx, ldq, scale_row, scale_block, cols};
+  const QuantArgs a{x, reinterpret_cast<unsigned char*>(q), scale, rows, ldx, ldq, scale_row, scale_block, cols, false};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define BY_TYPE(F)                                                                                          \
   (dtype == UNCL_F32 ? launch_quant<float, F>(a, tile, transposed, s)                                       \
@@ -259,7 +260,8 @@ extern "C" int uncl_quant8(const void* x, int dtype, long long rows, int cols, l
 // ---- the linear layer of a training step -----------------------------------------------------------------------------------------------
 // y = x w^T + b, gx = gy w, gw = gy^T x with 8-bit operands.  x and w are read once in the forward pass, for its own product (x by rows, w
 // by tiles) and, where gradients are wanted, for theirs (both transposed: a quarter to a half of the bytes that keeping x and w would
-// take); gy is read once in the backward pass for both products and the bias.
+// take); gy is read once in the backward pass for both products and the bias.  An infinity is quantised to NaN: as the largest number of its
+// block it would make finite results of a step that has overflowed, and a loss scale that looks for such steps would miss it.
 namespace {
 
 struct LinearPlan {                      // the operands' places in one buffer, 256-byte aligned
@@ -310,7 +312,7 @@ bool linear_ok(const uncl_linear8_desc* d) {
   return x && w && (d->grad_fmt == UNCL_E4M3 || d->grad_fmt == UNCL_E5M2);
 }
 QuantArgs quant_args(const void* x, long long rows, int cols, long long ldx, char* q, long long ldq, char* scale, long long row, long long blk) {
-  return {x, reinterpret_cast<unsigned char*>(q), reinterpret_cast<float*>(scale), rows, ldx, ldq, row, blk, cols};
+  return {x, reinterpret_cast<unsigned char*>(q), reinterpret_cast<float*>(scale), rows, ldx, ldq, row, blk, cols, true};
 }
 
 // x by rows and (t) by its columns' 128s; w by tiles, as it lies and (t) transposed; gy both ways and its columns' sums

@@ -142,7 +142,8 @@ __device__ __forceinline__ void ro_drop8(unsigned long long group, unsigned long
 
 // ---- 8-bit floating point (OCP e4m3fn / e5m2), blocks of 128 -------------------------------------------------------------------------
 // scale = max(amax, 2^-100) * fl(1 / top), inverse = fl(1 / scale), q = round_even(x * inverse) kept inside +-top.  amax is over the
-// FINITE values of the block: an infinity then becomes +-top, a NaN stays NaN, and neither reaches its neighbours.
+// FINITE values of the block: an infinity then becomes +-top (or NaN, where the caller asks for it), a NaN stays NaN, and neither reaches
+// its neighbours.
 #define RO_AMAX_MIN 7.8886090522101181e-31f   /* 2^-100: the scale of a block of zeros, its inverse finite */
 template <int FMT>
 struct RoF8 {
@@ -190,14 +191,15 @@ __device__ __forceinline__ float ro_scale_of(unsigned amax_bits) {
   return fmaxf(__builtin_bit_cast(float, amax_bits), RO_AMAX_MIN) * (1.0f / RoF8<FMT>::top);
 }
 // x / scale kept inside +-top, ready to be rounded (the quotient of a block's largest may be one fp32 step over top, which the conversion
-// would make a NaN)
+// would make a NaN).  lost: an infinity becomes a NaN instead (of the two formats one has no infinity), for a caller whose results must
+// not hide it.
 template <int FMT, bool ODD>
-__device__ __forceinline__ float ro_fit(float v, float inv) {
+__device__ __forceinline__ float ro_fit(float v, float inv, bool lost) {
 #pragma clang fp contract(off)
   const float q = v * inv;
   if (!ODD) return __builtin_amdgcn_fmed3f(q, -RoF8<FMT>::top, RoF8<FMT>::top);
   const float c = fminf(fmaxf(q, -RoF8<FMT>::top), RoF8<FMT>::top);
-  return q != q ? q : c;
+  return q != q || (lost && ro_size<false>(v) >= RO_INF_BITS) ? __builtin_nanf("") : c;
 }
 template <int FMT>
 __device__ __forceinline__ unsigned ro_pack4(float a, float b, float c, float d) {
@@ -212,14 +214,14 @@ __device__ __forceinline__ unsigned ro_pack4(float a, float b, float c, float d)
   return (unsigned)v;
 }
 template <int FMT>
-__device__ __forceinline__ u32x2 ro_pack8(const float* v, float inv, bool odd) {
+__device__ __forceinline__ u32x2 ro_pack8(const float* v, float inv, bool odd, bool lost = false) {
   float f[8];
   if (odd) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = ro_fit<FMT, true>(v[i], inv);
+    for (int i = 0; i < 8; ++i) f[i] = ro_fit<FMT, true>(v[i], inv, lost);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = ro_fit<FMT, false>(v[i], inv);
+    for (int i = 0; i < 8; ++i) f[i] = ro_fit<FMT, false>(v[i], inv, false);
   }
   return u32x2{ro_pack4<FMT>(f[0], f[1], f[2], f[3]), ro_pack4<FMT>(f[4], f[5], f[6], f[7])};
 }

@@ -523,8 +523,9 @@ def linear8(x, weight, bias=None, grad_fmt="e5m2"):
     """x weight^T + bias with all three products of a training step in 8 bits: x and weight are quantised to e4m3 (rows / tiles of 128), the
     gradient of the output to grad_fmt by rows -- along its columns for x's gradient, along its rows, like x, for weight's.  weight (N, K)
     fp32, bf16 or fp16; bias fp32 (N).  The result and x's gradient have x's type, weight's gradient weight's (summed in fp32).  The rounding
-    of the operands is not differentiated (straight through).  What the backward pass needs of x and weight is kept in 8 bits.  Up to 2^22
-    rows, channels and results (each is a common axis of one of the products)."""
+    of the operands is not differentiated (straight through).  What the backward pass needs of x and weight is kept in 8 bits.  An infinity in
+    x, weight or the gradient counts as NaN and makes NaN of every result it takes part in (a loss scale sees the step that overflowed); the
+    bias' gradient is the plain sum.  Up to 2^22 rows, channels and results (each is a common axis of one of the products)."""
     _need(x, "x", _DTYPES)
     rows, k = _extent(x)
     _need(weight, "weight", _DTYPES, None, x.device)
