@@ -57,3 +57,79 @@ def test_linear8_does_not_hide_an_overflow(m, n, k, dtype, fmt):
                 assert torch.equal(a[~h], b[~h]), (name, value, which)
     q = row_ops.quantize8(torch.full((1, 8), INF, device="cuda").index_fill(1, torch.tensor([1], device="cuda"), 2.0))      # quantize8 itself: the largest number
     assert torch.equal(q.values(), torch.full((1, 8), 2.0, device="cuda"))
+
+
+# ---- the large tiles with everything behind them ---------------------------------------------------------------------------------------
+def operand(rows, cols, block, fmt="e4m3", seed=0):
+    """a quantised matrix whose bytes behind a row's end are NaN"""
+    data, scale = R.quantize(rnd(rows, cols, seed=seed).cpu() * torch.exp2(torch.arange(cols) % 5 - 2.0), block, fmt)
+    room = torch.full((rows, -(-cols // 16) * 16 + 16), 0x7F, dtype=torch.uint8, device="cuda")
+    room[:, :cols] = data.view(torch.uint8).cuda()
+    return row_ops.Quant8(room.view(data.dtype)[:, :cols], scale.cuda(), block)
+
+
+def reference(a, b, dtype, bias=None, act="none", residual=None):
+    """64-bit value of a product and what may be off before the result's rounding; all on the GPU"""
+    want, size = R.matmul8(a, b)
+    tol = (128 + 8 + -(-a.data.shape[1] // 128)) * R.U * size + (R.cut(a, b) if dtype == torch.bfloat16 else 0.0)
+    if bias is not None:
+        want = want + bias.double()
+        tol = tol + R.U * (want.abs() + bias.double().abs())
+    if act == "relu":
+        want = want.clamp_min(0)
+    elif act == "gelu":
+        tol = 1.13 * tol + 16 * R.U * want.abs()                         # the slope is at most 1.13; erf and two products
+        want = want * torch.special.ndtr(want)
+    if residual is not None:
+        want = want + residual.double()
+        tol = tol + R.U * want.abs()
+    return want, tol
+
+
+def within(got, want, tol, dtype, what):
+    bad = (got.double() - want).abs() > tol + R.HALF[dtype] * (want.abs() + tol) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    assert not bad.any(), (what, int(bad.sum()), bad.nonzero()[0].tolist())
+
+
+# M, N and K with sides behind the last tile: 4101 x 3500 goes to 256 x 256 tiles where those are built (bf16 results, b by tiles), 2100 x 2050
+# to 128 x 128, 4099 rows leave three behind the last whole tile
+LARGE = [(4101, 3500, 1100), (2100, 2050, 384), (4099, 4096, 2048)]
+
+
+@pytest.mark.parametrize("m,n,k", LARGE)
+@pytest.mark.parametrize("block", ["tile", "row"])
+@pytest.mark.parametrize("fa", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_large_products_with_bias_activation_and_residual(m, n, k, block, fa, dtype):
+    a, b, bias = operand(m, k, "row", fa), operand(n, k, block, seed=1), rnd(n, seed=3)
+    res = rnd(m, n, dtype=dtype, seed=4, size=5.0)
+    for act in ("gelu", "relu"):
+        want, tol = reference(a, b, dtype, bias, act, res)
+        out = row_ops.matmul8(a, b, bias=bias, act=act, residual=res, out_dtype=dtype)
+        within(out, want, tol, dtype, act)
+    wide = torch.full((m, n + 9), 7.0, dtype=dtype, device="cuda")        # rows of a wider buffer at an odd address; what is beside stays
+    wide[:, 3:3 + n] = res
+    into = wide[:, 3:3 + n]
+    row_ops.matmul8(a, b, bias=bias, act=act, residual=into, out_dtype=dtype, out=into)                     # the residual is the result
+    assert torch.equal(into, out) and bool((wide[:, :3] == 7).all()) and bool((wide[:, 3 + n:] == 7).all())
+    pitched = torch.zeros(m, n + 5, dtype=dtype, device="cuda")[:, :n].copy_(res)
+    assert torch.equal(row_ops.matmul8(a, b, bias=bias, act=act, residual=pitched, out_dtype=dtype), out)
+
+
+@pytest.mark.parametrize("dtype,wtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32), (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("m,n,k", [(4099, 4096, 2048), (2100, 4096, 2050)])
+def test_large_linear8_with_all_gradients(m, n, k, dtype, wtype):
+    x, w, b, g = rnd(m, k, dtype=dtype), rnd(n, k, dtype=wtype, size=k ** -0.5, seed=1), rnd(n, seed=2), rnd(m, n, dtype=dtype, seed=3, size=0.01)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = row_ops.linear8(*leaves)
+    gx, gw, gb = torch.autograd.grad(y, leaves, g)
+
+    def q(t, block, fmt, tr=False):
+        return row_ops.Quant8(*(v.cuda() for v in R.quantize(t.cpu(), block, fmt, tr)), block)
+    for name, got, t, a, o, bias in (("y", y, dtype, q(x, "row", "e4m3"), q(w, "tile", "e4m3"), b), ("gx", gx, dtype, q(g, "row", "e5m2"), q(w, "tile", "e4m3", True), None),
+                                     ("gw", gw, wtype, q(g, "row", "e5m2", True), q(x, "row", "e4m3", True), None)):
+        want, tol = reference(a, o, t, bias)
+        assert got.dtype == t
+        within(got, want, tol, t, name)
+    bad = (gb.double() - g.double().sum(0)).abs() > 300 * R.U * g.double().abs().sum(0)       # 8 + 16 in a tile, two partial sums a lane, a fold of 32
+    assert not bad.any()
