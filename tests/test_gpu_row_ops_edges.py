@@ -133,3 +133,16 @@ def test_large_linear8_with_all_gradients(m, n, k, dtype, wtype):
         within(got, want, tol, t, name)
     bad = (gb.double() - g.double().sum(0)).abs() > 300 * R.U * g.double().abs().sum(0)       # 8 + 16 in a tile, two partial sums a lane, a fold of 32
     assert not bad.any()
+
+
+# ---- equal rows ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("m,n,k", [(4099, 4096, 2048), (4099, 2048, 4096), (4160, 4096, 1024), (300, 33000, 1024), (2100, 2050, 384), (28800, 256, 256)])
+@pytest.mark.parametrize("block", ["tile", "row"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_equal_rows_give_equal_results_wherever_they_stand(m, n, k, block, dtype):
+    """every row of a product is added up the same way: fifty rows over and over"""
+    a, b = operand(50, k, "row"), operand(n, k, block, seed=1)
+    i = torch.arange(m, device="cuda") % 50
+    many = row_ops.Quant8(a.data.view(torch.uint8)[i].view(a.data.dtype), a.scale[i], "row")
+    out = row_ops.matmul8(many, b, out_dtype=dtype)
+    assert torch.equal(out, out[:50][i])

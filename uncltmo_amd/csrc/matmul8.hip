@@ -115,13 +115,23 @@ int run_rows(const MmArgs& p, int a_fmt, bool tile, hipStream_t s) {
   return tile ? launch_rows<UNCL_E5M2, true>(p, s) : launch_rows<UNCL_E5M2, false>(p, s);
 }
 
-// Up to 64 rows behind the last whole 128 that would cost the tiles a round: a unit took 0.43 ns (bf16 results) or 0.73 ns a k in its ten
-// tenths, the few rows' kernel 4 us and b's bytes at 2.5 TB/s (4099 x 4096 x 2048: 51 us at once, 39 + 5 us in two).
-int ragged_rows(const MmArgs& p, bool large, bool exact) {
+// Up to 64 rows behind the last whole 128 that would cost the tiles a round, or the larger tiles: they go to small tiles of their own, in a
+// launch before the others.  (Not to the few rows' kernel, whose sums are the exact ones for every type: a row's result must not depend on its
+// place.)  That launch took 2.6 us and 3.3 (bf16 results) to 4.5 ns a k for 256 to 16384 columns; a unit took 0.25 to 0.39 ns a k in its ten
+// tenths (0.18 where the rest would change to smaller tiles: not then).  At once / apart, bf16 with b by tiles: 4099 x 4096 x 512 22.5 / 24.2,
+// x 1024 32.1 / 29.3, x 2048 52.7 / 46.0; 8195 x 4096 x 4096 158 / 133; 4099 x 16384 x 1024 101 / 91; 8195 x 1024 x 2048 30.6 / 32.7; fp32:
+// 4099 x 2048 x 1024 32.7 / 32.1, x 4096 94.8 / 86.8, 8195 x 4096 x 2048 149 / 148.
+int ragged_rows(const MmArgs& p, bool large) {
   const int tail = p.M & 127;
   if (p.M <= 128 || tail == 0 || tail > 64 || p.part) return 0;
-  const long long saved = mm_plan(p.M, p.N, p.KB, large).units - mm_plan(p.M - tail, p.N, p.KB, large).units;
-  return (double)saved * p.K * (exact ? 0.73 : 0.43) > 4000. + (double)p.N * p.K / 2500. ? tail : 0;
+  const MmPlan all = mm_plan(p.M, p.N, p.KB, large), rest = mm_plan(p.M - tail, p.N, p.KB, large);
+  const double rounds = (p.N + 65535ll) / 65536;              // of the small tiles, four to a CU
+  return rest.tile >= all.tile && (double)(all.units - rest.units) * p.K * 0.26 > rounds * (2600. + 4. * p.K) ? tail : 0;
+}
+
+int run_tiles(const MmArgs& p, int a_fmt, bool tile, hipStream_t s) {
+  if (p.out_dtype == UNCL_BF16) return mm_tiles_bf16(p, a_fmt, tile, s);
+  return p.out_dtype == UNCL_F16 ? mm_tiles_f16(p, a_fmt, tile, s) : mm_tiles_f32(p, a_fmt, tile, s);
 }
 
 }  // namespace
@@ -133,8 +143,7 @@ int mm_run(const MmArgs& args, int a_fmt, bool tile, void* workspace, hipStream_
   const int splits = workspace ? mm_splits(p.M, p.N, p.K) : 1;
   p.part = splits > 1 ? reinterpret_cast<float*>(workspace) : nullptr;
   p.per = (p.KB + splits - 1) / splits;
-  const bool exact = p.out_dtype != UNCL_BF16;
-  if (const int tail = ragged_rows(p, tile && !exact, exact)) {
+  if (const int tail = ragged_rows(p, tile && p.out_dtype == UNCL_BF16)) {
     MmArgs q = p;
     const long long at = p.M -= tail, e = p.out_dtype == UNCL_F32 ? 4 : 2;
     q.M = tail;
@@ -142,11 +151,10 @@ int mm_run(const MmArgs& args, int a_fmt, bool tile, void* workspace, hipStream_
     q.sa += at * p.sa_row;
     q.out = reinterpret_cast<char*>(p.out) + at * p.ldo * e;
     if (p.res) q.res = reinterpret_cast<const char*>(p.res) + at * p.ldr * e;
-    const int rc = run_rows(q, a_fmt, tile, s);
+    const int rc = run_tiles(q, a_fmt, tile, s);
     if (rc != UNCL_OK) return rc;
   }
-  if (!exact) return mm_tiles_bf16(p, a_fmt, tile, s);
-  return p.out_dtype == UNCL_F16 ? mm_tiles_f16(p, a_fmt, tile, s) : mm_tiles_f32(p, a_fmt, tile, s);
+  return run_tiles(p, a_fmt, tile, s);
 }
 
 extern "C" size_t uncl_matmul8_workspace_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? mm_split_bytes(M, N, K) : 0; }
