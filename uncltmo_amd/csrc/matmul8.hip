@@ -30,9 +30,9 @@ __device__ __forceinline__ void mm_store4(const MmArgs& p, long long m, int n, f
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------
 // Up to 64 rows: b is read once and is nearly all there is to read (so the sums are the exact ones for every type).  A workgroup owns 16
 // columns, its WAVES waves take the blocks of K in turn, operands come straight from global memory into registers, and the waves' sums
-// join in LDS in a fixed order.  1 x 4096 x 4096: 8.0 us, where 17 MB at the copy rate are 3.3: 256 workgroups, one a CU, with four blocks
-// in flight a wave -- a chain of about four round trips to memory, the join and the launch.
-template <int FA, bool BT, int TM, int WAVES, int UNROLL>
+// join in LDS in a fixed order.  1 x 4096 x 4096: 8.0 us, where 17 MB at the copy rate are 3.3: 256 workgroups, one a CU, eight waves with one
+// block each in flight -- four blocks a wave, so a chain of four round trips to memory, the join and the launch.
+template <int FA, bool BT, int TM, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void mm_rows_kernel(const MmArgs p) {
   __shared__ f32x4 red[WAVES][TM][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane & 15, g = lane >> 4;
@@ -50,7 +50,6 @@ __global__ __launch_bounds__(WAVES * 64) void mm_rows_kernel(const MmArgs p) {
   f32x4 acc[TM];
 #pragma unroll
   for (int i = 0; i < TM; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll UNROLL
   for (int kb = wave; kb < p.KB; kb += WAVES) {
     const int c0 = kb * 128 + g * 16, c1 = c0 + 64;
     const int r0 = c0 < last ? c0 : last, r1 = c1 < last ? c1 : last;
@@ -97,9 +96,9 @@ __global__ __launch_bounds__(WAVES * 64) void mm_rows_kernel(const MmArgs p) {
 template <int FA, bool BT>
 int launch_rows(const MmArgs& p, hipStream_t s) {
   const int grid = (p.N + 15) / 16;
-  if (p.M <= 16) mm_rows_kernel<FA, BT, 1, 8, 4><<<grid, 512, 0, s>>>(p);
-  else if (p.M <= 32) mm_rows_kernel<FA, BT, 2, 8, 2><<<grid, 512, 0, s>>>(p);
-  else mm_rows_kernel<FA, BT, 4, 8, 2><<<grid, 512, 0, s>>>(p);
+  if (p.M <= 16) mm_rows_kernel<FA, BT, 1, 8><<<grid, 512, 0, s>>>(p);
+  else if (p.M <= 32) mm_rows_kernel<FA, BT, 2, 8><<<grid, 512, 0, s>>>(p);
+  else mm_rows_kernel<FA, BT, 4, 8><<<grid, 512, 0, s>>>(p);
   UNCL_CHECK_LAUNCH();
   return UNCL_OK;
 }
