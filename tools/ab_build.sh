@@ -6,6 +6,7 @@ ROOT=$(cd "$(dirname "$0")/.." && pwd)
 C=$1; NAME=$2
 TMP=$(mktemp -d)
 git -C "$ROOT" archive "$C" uncltmo_amd/csrc include | tar -x -C "$TMP"
-/opt/rocm/bin/hipcc -O3 --offload-arch=gfx950 -fPIC -shared -I"$TMP/include" -I"$TMP/uncltmo_amd/csrc" -o "$ROOT/tools/_ab/lib$NAME.so" "$TMP"/uncltmo_amd/csrc/*.hip
+mkdir -p "$ROOT/tools/_ab"
+/opt/rocm/bin/hipcc $(python3 "$ROOT/__graft_entry__.py" flags) -shared -I"$TMP/include" -I"$TMP/uncltmo_amd/csrc" -o "$ROOT/tools/_ab/lib$NAME.so" "$TMP"/uncltmo_amd/csrc/*.hip
 rm -rf "$TMP"
 echo built tools/_ab/lib$NAME.so

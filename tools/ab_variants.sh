@@ -8,13 +8,14 @@ set -e
 FILES=${FILES:-"conv3x3_pc conv3x3_pipe"}
 ROOT=$(cd "$(dirname "$0")/.." && pwd)
 mkdir -p "$ROOT/tools/_ab" "$ROOT/build/ab"
+BASE=$(python3 "$ROOT/__graft_entry__.py" flags)
 pids=()
 names=()
 while [ $# -ge 2 ]; do
   NAME=$1; FLAGS=$2; shift 2
   names+=("$NAME")
   for f in $FILES; do
-    /opt/rocm/bin/hipcc -O3 --offload-arch=gfx950 -fPIC -std=c++17 $FLAGS -c "$ROOT/uncltmo_amd/csrc/$f.hip" -o "$ROOT/build/ab/$f.$NAME.o" 2>/dev/null &
+    /opt/rocm/bin/hipcc $BASE $FLAGS -c "$ROOT/uncltmo_amd/csrc/$f.hip" -o "$ROOT/build/ab/$f.$NAME.o" 2>/dev/null &
     pids+=($!)
   done
 done

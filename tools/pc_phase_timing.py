@@ -14,6 +14,8 @@ import sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 
+from __graft_entry__ import FLAGS  # noqa: E402
+
 CONS = ["MFMA phase", "epilogue", "barrier wait", "-"]
 PROD = ["-", "register wait + LDS staging", "cursor + load issue", "barrier wait"]
 
@@ -23,7 +25,7 @@ def build():
     os.makedirs(out, exist_ok=True)
     lib = os.path.join(out, "libuncltmo_hip_pct.so")
     srcs = sorted(glob.glob(os.path.join(ROOT, "uncltmo_amd", "csrc", "*.hip")))
-    deps = srcs + glob.glob(os.path.join(ROOT, "uncltmo_amd", "csrc", "*.h"))
+    deps = srcs + glob.glob(os.path.join(ROOT, "uncltmo_amd", "csrc", "*.h")) + [os.path.join(ROOT, "__graft_entry__.py")]
     if os.path.exists(lib) and all(os.path.getmtime(lib) > os.path.getmtime(s) for s in deps):
         return lib
     objs, procs = [], []
@@ -31,7 +33,7 @@ def build():
         o = os.path.join(out, os.path.basename(s) + ".pct.o")
         objs.append(o)
         extra = os.environ.get("UNCL_PC_BUILD_FLAGS", "").split()
-        procs.append(subprocess.Popen(["/opt/rocm/bin/hipcc", "-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-DUNCL_PC_TIMING",
+        procs.append(subprocess.Popen(["/opt/rocm/bin/hipcc", *FLAGS, "-DUNCL_PC_TIMING",
                                        *extra, "-c", s, "-o", o]))
     for p in procs:
         if p.wait() != 0:

@@ -14,6 +14,8 @@ import sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 
+from __graft_entry__ import FLAGS  # noqa: E402
+
 PHASES = ["cursor+prefetch issue", "MFMA phase", "barrier(before epilogue)", "epilogue LDS transpose+barrier",
           "global stores issue", "end-of-step barrier", "vmcnt(0) wait", "LDS staging writes", "barrier(after staging)"]
 
@@ -23,9 +25,9 @@ def build(extra=()):
     os.makedirs(out, exist_ok=True)
     lib = os.path.join(out, "libuncltmo_hip_timing%s.so" % ("_fi" if extra else ""))
     srcs = sorted(glob.glob(os.path.join(ROOT, "uncltmo_amd", "csrc", "*.hip")))
-    if os.path.exists(lib) and all(os.path.getmtime(lib) > os.path.getmtime(s) for s in srcs):
+    if os.path.exists(lib) and all(os.path.getmtime(lib) > os.path.getmtime(s) for s in srcs + [os.path.join(ROOT, "__graft_entry__.py")]):
         return lib
-    cmd = ["/opt/rocm/bin/hipcc", "-O3", "--offload-arch=gfx950", "-fPIC", "-shared", "-DUNCL_PIPE_TIMING", *extra,
+    cmd = ["/opt/rocm/bin/hipcc", *FLAGS, "-shared", "-DUNCL_PIPE_TIMING", *extra,
            "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROOT, "uncltmo_amd", "csrc"), "-o", lib] + srcs
     subprocess.check_call(cmd)
     return lib
