@@ -146,3 +146,38 @@ def test_equal_rows_give_equal_results_wherever_they_stand(m, n, k, block, dtype
     many = row_ops.Quant8(a.data.view(torch.uint8)[i].view(a.data.dtype), a.scale[i], "row")
     out = row_ops.matmul8(many, b, out_dtype=dtype)
     assert torch.equal(out, out[:50][i])
+
+
+# ---- the longest grids -----------------------------------------------------------------------------------------------------------------
+LONG = 2 ** 27 + 128 + 40                     # columns: a workgroup of 512 threads for each sixteen is more than 2^32 threads
+
+
+@pytest.mark.parametrize("block", ["tile", "row"])
+def test_a_product_of_few_rows_and_over_2_to_the_27_columns(block):
+    m, k = 2, 16
+    g = torch.Generator(device="cuda").manual_seed(3)
+    a = row_ops.Quant8(torch.randint(0, 0x78, (m, k), dtype=torch.uint8, device="cuda", generator=g).view(torch.float8_e4m3fn), torch.ones(m, 1, device="cuda"), "row")
+    b = row_ops.Quant8(torch.randint(0, 0x78, (LONG, k), dtype=torch.uint8, device="cuda", generator=g).view(torch.float8_e4m3fn),
+                       1 + torch.rand(LONG if block == "row" else (LONG + 127) // 128, 1, device="cuda", generator=g), block)
+    bias, res = torch.randn(LONG, device="cuda", generator=g), torch.randn(m, LONG, device="cuda", generator=g)
+    out = row_ops.matmul8(a, b, bias=bias, residual=res, out_dtype=torch.float32)
+    for first in (0, 2 ** 26 - 256, 2 ** 26, 2 ** 27 - 256, 2 ** 27, 2 ** 27 + 128):             # (whole tiles of 128, so that scales go with them)
+        n = slice(first, min(first + 256, LONG))
+        part = row_ops.Quant8(b.data[n], b.scale[n if block == "row" else slice(n.start // 128, (n.stop + 127) // 128)], block)
+        want, size = R.matmul8(a, part)
+        tol = 137 * R.U * (size + bias[n].double().abs() + res[:, n].double().abs())
+        assert first % 128 == 0
+        within(out[:, n], want + bias[n].double() + res[:, n].double(), tol, torch.float32, first)
+
+
+def test_a_weights_gradient_of_over_2_to_the_27_channels():
+    """rows of ones of both signs: their mean square is exactly 1"""
+    x = torch.ones(2, LONG, dtype=torch.bfloat16, device="cuda")
+    x[:, ::3] = -1
+    gy = rnd(2, LONG, dtype=torch.bfloat16)
+    w = torch.ones(LONG, device="cuda", requires_grad=True)
+    y = row_ops.rms_norm(x, w, 1e-6)
+    assert bool((y == x).all())                                              # 1 - 5e-7 rounds to 1
+    gw, = torch.autograd.grad(y, [w], gy)
+    want = (gy.float() * x.float()).sum(0)                                   # exact but for one rounding
+    assert bool(((gw - want).abs() <= 1e-6 * gy.float().abs().sum(0)).all())

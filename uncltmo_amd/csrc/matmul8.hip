@@ -93,13 +93,25 @@ __global__ __launch_bounds__(WAVES * 64) void mm_rows_kernel(const MmArgs p) {
   }
 }
 
+// a grid's axis holds under 2^32 threads (2^27 columns, sixteen to a workgroup of 512; more wrap round without an error): in parts
+constexpr int ROWS_PART = 1 << 26;
 template <int FA, bool BT>
-int launch_rows(const MmArgs& p, hipStream_t s) {
-  const int grid = (p.N + 15) / 16;
-  if (p.M <= 16) mm_rows_kernel<FA, BT, 1, 8><<<grid, 512, 0, s>>>(p);
-  else if (p.M <= 32) mm_rows_kernel<FA, BT, 2, 8><<<grid, 512, 0, s>>>(p);
-  else mm_rows_kernel<FA, BT, 4, 8><<<grid, 512, 0, s>>>(p);
-  UNCL_CHECK_LAUNCH();
+int launch_rows(const MmArgs& args, hipStream_t s) {
+  const int e = args.out_dtype == UNCL_F32 ? 4 : 2;
+  for (int n = 0; n < args.N; n += ROWS_PART) {
+    MmArgs p = args;
+    p.N = args.N - n < ROWS_PART ? args.N - n : ROWS_PART;
+    p.b += n * p.ldb;
+    p.sb += BT ? (n >> 7) * p.sb_row : n;
+    if (p.bias) p.bias += n;
+    if (p.res) p.res = reinterpret_cast<const char*>(p.res) + (long long)n * e;
+    p.out = reinterpret_cast<char*>(p.out) + (long long)n * e;
+    const int grid = (p.N + 15) / 16;
+    if (p.M <= 16) mm_rows_kernel<FA, BT, 1, 8><<<grid, 512, 0, s>>>(p);
+    else if (p.M <= 32) mm_rows_kernel<FA, BT, 2, 8><<<grid, 512, 0, s>>>(p);
+    else mm_rows_kernel<FA, BT, 4, 8><<<grid, 512, 0, s>>>(p);
+    UNCL_CHECK_LAUNCH();
+  }
   return UNCL_OK;
 }
 
@@ -170,7 +182,7 @@ extern "C" int uncl_matmul8(const uncl_matmul8_desc* d, void* workspace, void* s
     return UNCL_ERR_ARG;
   if (!d->b_tile && d->b_scale_row != 1 && d->N > 1) return UNCL_ERR_ARG;
   if (d->ldo < d->N || (d->res && d->ldr < d->N)) return UNCL_ERR_ARG;
-  if ((long long)((d->M + 63) / 64) * ((d->N + 63) / 64) > 0x7fffffffll) return UNCL_ERR_ARG;
+  if (mm_tiles(d->M, d->N, 128) >= 1 << 24) return UNCL_ERR_ARG;      // one workgroup of 256 threads each, under 2^32 in all
   MmArgs p{};
   p.a = reinterpret_cast<const unsigned char*>(d->a); p.b = reinterpret_cast<const unsigned char*>(d->b);
   p.sa = d->a_scale; p.sb = d->b_scale; p.bias = d->bias; p.res = d->res; p.out = d->out;
