@@ -103,3 +103,18 @@ def test_quantised_tiles_have_a_limit_of_rows(calls):
             row_ops.quantize8(meta(most + 1, 8), **kw)
     row_ops.quantize8(meta(most + 1, 8))
     assert calls == ["uncl_quant8"] * 4
+
+
+def test_layouts_that_the_product_does_not_read_are_copied(calls, monkeypatch):
+    """one row whose stride is any number, and rows far apart: taken like every other layout, within the entry's limits"""
+    sent = []
+    monkeypatch.setattr(row_ops, "_call", lambda dev, what, fn, desc, *args: sent.append({k: getattr(desc._obj, k) for k in ("M", "lda", "ldb", "a_scale_row", "b_scale_row")}))
+    b = q8(8, 256, "tile")
+    far = meta(2 ** 21 * 2, 2, dtype=torch.float32).as_strided((1, 2), (2 ** 21, 1))
+    row_ops.matmul8(row_ops.Quant8(q8(1, 256, "row").data, far, "row"), b)                       # scales of one row
+    row_ops.matmul8(q8(1, 256, "row"), row_ops.Quant8(b.data, far, "tile"))
+    row_ops.matmul8(q8(3, 256, "row", 2 ** 22 + 16), b)                                          # rows of a and of b
+    row_ops.matmul8(q8(3, 256, "row"), q8(8, 256, "tile", 2 ** 22 + 16))
+    assert len(sent) == 4
+    for d in sent:
+        assert d["lda"] <= 2 ** 22 and d["ldb"] <= 2 ** 22 and 0 <= d["a_scale_row"] <= 2 ** 20 and 0 <= d["b_scale_row"] <= 2 ** 20, d

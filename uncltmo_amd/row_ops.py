@@ -374,10 +374,11 @@ def quantize8(x, block="row", transpose=False, fmt="e4m3"):
 
 
 def _operand(t):
-    """8-bit rows as the product reads them: on 16-byte borders, readable up to the next one behind a row's end; (tensor, pitch)"""
+    """8-bit rows as the product reads them: on 16-byte borders, at most 2^22 bytes apart, readable up to the next one behind a row's end; (tensor,
+    pitch)"""
     (rows, cols), (pitch, step) = t.shape, t.stride()
     room = (cols + 15) & ~15
-    if (step == 1 or cols == 1) and pitch >= cols and pitch % 16 == 0 and t.data_ptr() % 16 == 0 and (
+    if (step == 1 or cols == 1) and pitch >= cols and pitch % 16 == 0 and pitch <= 1 << 22 and t.data_ptr() % 16 == 0 and (
             pitch >= room and t.storage_offset() + (rows - 1) * pitch + room <= t.untyped_storage().nbytes()):
         return t, pitch
     out = torch.zeros(rows, room, dtype=torch.uint8, device=t.device)
@@ -387,6 +388,8 @@ def _operand(t):
 
 def _scale(t, most=1 << 20):
     """block scales with rows as near as the product wants them, within 32-bit offsets or neighbours; (tensor, its two strides)"""
+    if t.shape[0] == 1:                                      # (whatever a single row's stride says)
+        return t, (1, t.stride(1))
     if not (1 if most == 1 else 0) <= t.stride(0) <= most:
         t = t.t().contiguous().t()
     return t, t.stride()
