@@ -118,3 +118,13 @@ def test_layouts_that_the_product_does_not_read_are_copied(calls, monkeypatch):
     assert len(sent) == 4
     for d in sent:
         assert d["lda"] <= 2 ** 22 and d["ldb"] <= 2 ** 22 and 0 <= d["a_scale_row"] <= 2 ** 20 and 0 <= d["b_scale_row"] <= 2 ** 20, d
+
+
+def test_scales_that_want_a_gradient_are_refused(calls):
+    a, b = row_ops.Quant8(torch.ones(4, 16).to(E4M3), torch.ones(4, 1), "row"), row_ops.Quant8(torch.ones(16, 16).to(E4M3), torch.ones(1, 1), "tile")
+    for qa, qb in ((a._replace(scale=torch.ones(4, 1, requires_grad=True)), b), (a, b._replace(scale=torch.ones(1, 1, requires_grad=True)))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            row_ops.matmul8(qa, qb)
+        with torch.no_grad():
+            row_ops.matmul8(qa, qb)
+    assert calls == ["uncl_matmul8"] * 2

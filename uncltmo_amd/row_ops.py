@@ -434,6 +434,7 @@ def matmul8(a, b, bias=None, act="none", residual=None, out_dtype=torch.bfloat16
     if residual is not None:
         _need(residual, "residual", (out_dtype,), (m, n), dev)
     _no_grad("matmul8", bias, residual, out)
+    _no_grad("matmul8", a.scale, b.scale)
     given = out is not None
     if not given:
         out, ldo = torch.empty(m, n, dtype=out_dtype, device=dev), n
