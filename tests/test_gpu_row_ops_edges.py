@@ -181,3 +181,27 @@ def test_a_weights_gradient_of_over_2_to_the_27_channels():
     gw, = torch.autograd.grad(y, [w], gy)
     want = (gy.float() * x.float()).sum(0)                                   # exact but for one rounding
     assert bool(((gw - want).abs() <= 1e-6 * gy.float().abs().sum(0)).all())
+
+
+# ---- rows whose squares leave fp32 -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("cols", [5, 13, 32, 64, 300, 1000, 3000, 8200, 20001])
+def test_norm_of_large_values(cols, dtype):
+    """tolerances as for other rows (test_gpu_row_ops): scaling by a power of two rounds nothing"""
+    x, gy, w = rnd(12, cols, dtype=dtype), rnd(12, cols, dtype=dtype, seed=1), 1 + 0.1 * rnd(cols, seed=2)
+    size = torch.tensor([1.0, 2.0 ** 62, 2.0 ** 64, 2.0 ** 66, 1.0, 2.0 ** 90, 2.0 ** 120, 1.0, 2.0 ** 64, 2.0 ** -20, 2.0 ** 118, 2.0 ** 70], device="cuda")
+    x = (x.float() * size[:, None]).to(dtype)
+    x[4, 1] = INF
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = row_ops.rms_norm(xs, ws, 1e-6)
+    gx, gw = torch.autograd.grad(y, [xs, ws], gy)
+    ok = torch.arange(12, device="cuda") != 4
+    want, _ = R.norm(x[ok], w, 1e-6)
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    assert bool(((y[ok].double() - want).abs() <= (R.HALF[dtype] + 96 * R.U) * want.abs() + tiny).all())
+    assert bool(torch.isnan(y[4, 1])) and bool((y[4, torch.arange(cols, device="cuda") != 1] == 0).all())
+    want, size, _, _ = R.norm_backward(gy[ok], None, x[ok], w, 1e-6)
+    assert bool(((gx[ok].double() - want).abs() <= R.HALF[dtype] * want.abs() + 128 * R.U * size + 2 * tiny).all())
+    q, _ = row_ops.rms_norm_quant8(x, w)
+    q1, _ = row_ops.rms_norm_quant8((x.float() * torch.where(x.float().abs().amax(1) > 2.0 ** 40, 2.0 ** -60, 1.0)[:, None]).to(dtype), w)
+    assert bool(((q.values()[ok] - q1.values()[ok]).abs() <= 2.0 ** -3 * q1.values()[ok].abs() + 2.0 ** -8 * q1.scale.amax()).all())

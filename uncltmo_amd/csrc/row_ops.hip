@@ -45,6 +45,15 @@ __device__ __forceinline__ float row_sum(float v, float* red, int& turn) {
   return v;
 }
 
+// Squares of values over about 2^63 leave fp32's range: the sum is then infinite, and is made again from 2^-64 of the values.  again: that sum
+// over the row (infinite still where a value is)
+#define RO_FAR 0x1p-64f
+template <typename F>
+__device__ __forceinline__ float inverse_rms(float sum, float inv_cols, float eps, F again) {
+  if (__builtin_expect(sum == __builtin_inff(), 0)) return rsqrtf(again() * inv_cols + eps * (RO_FAR * RO_FAR)) * RO_FAR;
+  return rsqrtf(sum * inv_cols + eps);
+}
+
 // FMT: UNCL_Q8_NONE = y in T; UNCL_E4M3 / UNCL_E5M2 = y in 8 bits with a scale for each 128 channels (sixteen lanes hold one block)
 template <typename T, int LANES, int CH, int FMT>
 __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a) {
@@ -90,7 +99,14 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum = i < n ? fmaf(v[c][i], v[c][i], sum) : sum;
     }
-    const float r = rsqrtf(row_sum<LANES>(sum, red, turn) * a.inv_cols + a.eps);
+    const float r = inverse_rms(row_sum<LANES>(sum, red, turn), a.inv_cols, a.eps, [&]() {
+      float far = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) far = fmaf(v[c][i] * RO_FAR, v[c][i] * RO_FAR, far);        // (0 behind the row's end)
+      return row_sum<LANES>(far, red, turn);
+    });
     if (a.rstd && live && lane == 0) a.rstd[row] = r;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -141,7 +157,16 @@ __global__ __launch_bounds__(256) void norm_long_kernel(const NormArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum = i < a.cols - col ? fmaf(v[i], v[i], sum) : sum;
     }
-    const float r = rsqrtf(row_sum<256>(sum, red, turn) * a.inv_cols + a.eps);
+    const float r = inverse_rms(row_sum<256>(sum, red, turn), a.inv_cols, a.eps, [&]() {
+      float far = 0.f;
+      for (int col = threadIdx.x * 8; col < a.cols; col += 2048) {
+        float v[8];
+        sum8(col, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) far = i < a.cols - col ? fmaf(v[i] * RO_FAR, v[i] * RO_FAR, far) : far;
+      }
+      return row_sum<256>(far, red, turn);
+    });
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = r;
     // whole waves stay in the loop: sixteen lanes share a block's maximum.  h is written here, behind the last read of x and res by
     // this thread, so that it may be one of them
