@@ -109,6 +109,13 @@ __device__ __forceinline__ int mm_turn(int row) { return (row >> 1) & 7; }
 // everything this wave has in flight has arrived, and every wave of the workgroup says so
 __device__ __forceinline__ void mm_arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// The lanes of a wave hand numbers to each other through its own part of LDS: the hardware keeps a wave's LDS operations in order, this keeps the
+// compiler's (which sees one thread) in that order too.  No instruction.
+__device__ __forceinline__ void mm_wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // bytes from a row of a matrix on, bounds-checked by the hardware: `rows` rows `pitch` bytes apart, `len` bytes of each
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mm_buffer(const void* p, long long rows, long long pitch, long long len) {
   const long long n = (rows - 1) * pitch + len;
@@ -367,6 +374,7 @@ __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(w + (i * 16 + q) * PITCH + j * 16 + g * 4) = acc[j][ch * 2 + i];
+        mm_wave_order();
 #pragma unroll
         for (int t = 0; t < PASSES; ++t) {
           const int m = mb + ch * 32 + t * RPP + r0;
@@ -377,6 +385,7 @@ __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(
             *reinterpret_cast<f32x4*>(part + (long long)m * n8 + 4) = hi;
           }
         }
+        mm_wave_order();
       }
       return;
     }
@@ -409,6 +418,7 @@ __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(w + (i * 16 + q) * PITCH + j * 16 + g * 4) = acc[j][ch * 2 + i];
+    mm_wave_order();
 #pragma unroll
     for (int t = 0; t < PASSES; ++t) {
       const int m = mb + ch * 32 + t * RPP + r0;
@@ -423,6 +433,7 @@ __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(
         for (int e = 0; e < 8; ++e) v[e] += r[t][e];
       if (m < p.M && left > 0) ro_store8(out + (long long)m * p.ldo + n, left, v);
     }
+    mm_wave_order();
   }
 }
 
