@@ -808,9 +808,10 @@ int uncl_quant8(const void* x, int dtype, long long rows, int cols, long long ld
  * (a e4m3 or e5m2, b e4m3), any M and N, K to 2^22; rows start on 16-byte borders (pointers and lda / ldb multiples of 16 bytes, at most
  * 2^22) and are readable up to the next multiple of 16 bytes behind K (what stands there has no effect).  a_scale[m * a_scale_row + kb *
  * a_scale_block]; b_scale likewise by n (b_tile = 0) or n / 128 (b_tile = 1); distances between rows of scales 0 to 2^20, 1 for b's with b_tile = 0.  bias fp32 [N] or NULL; act UNCL_ACT_*; res (type of out) or NULL, may be out.  Sums are fp32, in an order that
- * depends on the sizes and types alone.  With a bf16 result and over 64 rows, products are added up by the 8-bit matrix instruction, which
- * cuts each off 13 bits under the largest power of two among its eight neighbours along k: about 1e-4 of the result, a tenth of its
- * rounding.  fp16 and fp32 results do without that. */
+ * depends on the sizes and types alone, the same for every row.  With a bf16 result and over 64 rows, products are added up by the 8-bit matrix
+ * instruction, which cuts each off 13 bits under the largest power of two among its eight neighbours along k: at most 7 x 2^-13 of each
+ * eight's largest product, added up (normal operands: 1.4e-5 of the results' rms, at most 1.3e-4, under a bf16 rounding of 1.7e-3; of a result
+ * that cancels it may be any part).  fp16 and fp32 results do without that: ask for fp32 where it matters. */
 typedef struct uncl_matmul8_desc {
   int M, N, K;
   int a_fmt, b_fmt, b_tile;

@@ -495,7 +495,7 @@ __global__ __launch_bounds__((4 + PW) * 64, PW == 8 ? 3 : (NT == 1 && MPW == 2 ?
     };
 
     // The forward epilogue (bias + ReLU, plain store, optional pooled copy) with nothing in it that is not arithmetic on
-    // packed registers: 32 v_pk_add_f32 + 32 v_cvt_pk + 16 v_permlane32_swap + 32 v_pk_max_i16 per 64 accumulators, stores
+    // packed registers: 64 v_add_f32 + 32 v_cvt_pk + 16 v_permlane32_swap + 32 v_pk_max_i16 per 64 accumulators, stores
     // as "scalar row base + 32-bit lane offset + immediate".  The generic form above costs 3-7x the instructions (64-bit
     // per-lane addresses, per-element selects, float round trips in the pooled copy) and was half of a 64-channel tile's time.
     typedef float f32x2 __attribute__((ext_vector_type(2)));

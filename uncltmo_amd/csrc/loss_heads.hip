@@ -1022,15 +1022,15 @@ __global__ __launch_bounds__(NWAVE * 64) void gauss_stats_bwd32_kernel(const bf1
 // three, and the inputs of a run of four outputs read as 12 dwords (two 16-bit pixels each) instead of 14 single elements.
 // Interior tiles take the weights from scalar registers; a tile that touches an end of the axis reads a per-position row from
 // a small LDS table built at the start.  A wave works on TWO of its channels at a time (288 + 128 units over 64 lanes).
-// Measured (8 samples): 148 -> 144 us with scalar multiply-adds, 137 with the packed ones of gc_taps4 -- of which 42 us are the
-// load and store phases (-DUNCL_GC_ABL=1); the rest is instruction issue at two waves per SIMD (the planes' 44 KB per workgroup
-// allow no third workgroup per CU).
+// Measured: 148 us for four passes, 133 in this form at 8 samples, 481 at 32 (a call in a row; every multiply-add a scalar one) -- of which
+// 42 us at 8 samples are the load and store phases (-DUNCL_GC_ABL=1); the rest is instruction issue at two waves per SIMD (the planes'
+// 44 KB per workgroup allow no third workgroup per CU).
 struct GaussC { float c[2 * GW - 1]; float bt[GW - 1][2 * GW - 1]; };
 constexpr int CT = 2 * GW - 1 /*21 taps*/, CTP = 20 /*row pitch of the intermediate in floats: 4 CTP = 16 (mod 64) banks per run of rows*/;
 constexpr int GC_T = 2 * HI * CTP;             // floats of intermediate per wave (two channels)
-// four outputs of a 21-tap filter from 24 inputs: out[r] = sum_t w[t] in[r + t].  Packed fp32 multiply-adds on the ALIGNED input
-// pairs (in[2k], in[2k+1]) only: an even tap feeds output pairs (0,1), (2,3); an odd tap the pair (1,2) plus two single
-// multiply-adds for outputs 0 and 3 -- 52 instructions instead of 84.  Even and odd taps accumulate separately (fixed order).
+// four outputs of a 21-tap filter from 24 inputs: out[r] = sum_t w[t] in[r + t].  Even and odd taps accumulate separately (fixed order), in
+// pairs of outputs that start on even inputs: an even tap feeds (0,1), (2,3); an odd tap (1,2), and 0 and 3 by themselves.  84 multiply-adds:
+// the build keeps packed fp32 arithmetic, which the pairs were laid out for, out of all GPU code.
 typedef float gc_f2 __attribute__((ext_vector_type(2)));
 template <typename WF>
 __device__ __forceinline__ void gc_taps4(const float (&in)[24], WF w, float (&out)[4]) {

@@ -10,9 +10,12 @@
 //
 // Two ways to add up a block.  The 8-bit instruction (16x16x128) adds products eight at a time on a common exponent and cuts each of them
 // off 13 bits under the largest power of two in its group (measured, the same for all of the card's 8-bit forms; between groups it adds
-// in fp32): about 1e-4 of a result of random signs.  That is a tenth of a rounding to bf16, so results in bf16 take it.  Results in fp16
-// and fp32 would show it: there the operands are widened to bf16 in registers (exact: three or four significant bits, any exponent) and
-// go through the bf16 instruction, whose sums measured 2^-23 of the products' sizes, at half the rate.
+// in fp32): at most 7 x 2^-13 of the groups' largest products, added up.  Normal operands, K = 256 to 8192: 1.4e-5 of the results' rms, at
+// most 1.3e-4; positive ones 3.6e-6 of the result.  That is a hundredth of a rounding to bf16 (1.7e-3), so results in bf16 take it: one to
+// three in a hundred of them round the other way, and their distance from the 64-bit value is that of the fp32 sum's rounding to four digits.
+// It goes with the PRODUCTS' sizes: of a result that cancels it may be any part.  Results in fp16 and fp32 would show it: there the operands
+// are widened to bf16 in registers (exact: three or four significant bits, any exponent) and go through the bf16 instruction, whose sums
+// measured 2^-23 of the products' sizes, at half the rate.
 #pragma once
 #include "matmul8_args.h"
 #include "row_ops.h"
@@ -89,7 +92,7 @@ __device__ __forceinline__ float mm_gelu(float x) {
 // the rarer activations, one copy of their code
 __device__ __attribute__((noinline)) float mm_act_rare(float v, int act) { return uncl_act(v, act); }
 
-// eight neighbouring columns from n on of row m (`left` of them exist): act(v + bias) + residual, rounded once
+// the activation of E sums
 template <int E>
 __device__ __forceinline__ void mm_act(float* v, int act) {
   if (act == UNCL_ACT_GELU) {
@@ -126,9 +129,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mm_buffer(const void* p, long 
 // A workgroup of WM x WN waves owns BM x BN outputs; a stage of LDS holds 128 bytes of each of its BM + BN rows, two stages.  Rows
 // come in by asynchronous 16-byte loads straight to LDS, a block ahead of the products, and the block's scales with them: one barrier
 // a block says both that this block has arrived and that nobody reads the stage that the next one overwrites.  Chunk c of row r lies at
-// position c ^ mm_turn(r), so that the rows that a part of a wave reads at once fall on different banks (no conflicts are counted).  The loads write LDS in
-// lane order, hence the swizzle is in the lane's global address.  Rows behind M or N are out of the buffers' bounds (their results are not
-// stored); bytes behind K, of the next row or out of bounds, are cleared in LDS.
+// position c ^ mm_turn(r), so that the rows that a part of a wave reads at once fall on different banks (conflicts counted: 256 cycles a
+// workgroup of 128 x 128 at K = 256 and at 4096 alike, all of them where the results turn round at the end).  The loads write LDS in lane order,
+// hence the swizzle is in the lane's global address.  Rows behind M or N are out of the buffers' bounds (their results are not stored);
+// bytes behind K, of the next row or out of bounds, are cleared in LDS.
 //
 // Workgroups go to the card's eight XCDs in turn, each with an L2 of its own: the b-th workgroup takes the (b / 8)-th tile of its XCD's
 // share, and a share runs through groups of eight rows of tiles, so that the 32 tiles at work on an XCD have few rows and columns.
@@ -393,8 +397,8 @@ __global__ __launch_bounds__(WM * WN * 64, BM > 64 ? 2 : 4) void mm_tile_kernel(
 #pragma unroll
   for (int e = 0; e < 8; ++e) bias[e] = 0.f;
   if (p.bias && left > 0) ro_load8(p.bias + n, left, bias);
-  // Where all columns exist the residual's loads need no branches and go out together (bf16, 8192 x 4096 x 4096 135 -> 130 us, 28800 x
-  // 1024 x 256 34 -> 29.5).  Rows behind M read the last one again, for nothing.
+  // Where all columns exist the residual's loads need no branches and go out together (bf16, inputs of four sets in turn: 8192 x 4096 x 4096
+  // 153 -> 146 us, 28800 x 1024 x 256 47 -> 36).  Rows behind M read the last one again, for nothing.
   const bool whole = res && nb + COLS <= p.N;
 #pragma unroll
   for (int ch = 0; ch < TM / 2; ++ch) {

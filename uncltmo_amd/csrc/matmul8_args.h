@@ -20,7 +20,11 @@ static inline long long mm_tiles(int M, int N, int t) { return (long long)((M + 
 // tiles (8-bit instruction, b scaled by tiles) work one to a CU, four units a round; 128 x 128 ones two to a CU, two units a round, a
 // tenth slower a unit (8192 x 4096 x 4096: 124 against 146 us; 4099 x 4096 x 2048, 8 units against 6: 65 against 51 us; a short K leaves
 // nothing to hide the epilogue behind but another workgroup: 28800 x 1024 x 256 with GELU 35.8 against 33.4 us).  64 x 64 tiles, four to a CU,
-// where 128 x 128 ones are at most one a CU (512 x 4096 x 4096: 19 against 27 us; 2048 x 2048 x 2048 17.2 against 17.7).
+// where 128 x 128 ones are at most one a CU (512 x 4096 x 4096: 19 against 27 us; 2048 x 2048 x 2048 16.4 against 16.0, x 512 8.2 against 8.1).
+// All three at 14 outputs from 1024 x 1024 to 28800 x 1024 and K = 128 to 4096, without bias: for bf16 results the rule's tiles are the fastest or
+// within 10 % of them, but for 256 x 256 ones under K = 768 (4096 x 4096 x 512: 16.0 against the chosen 17.9, 8192 x 2048 x 512 15.7 against
+// 17.9); for exact sums 64 x 64 ones would be up to 20 % faster at 257 to 320 large tiles (2304 x 2048 x 1024: 18.0 against the chosen 21.7) and
+// up to a third at K = 128 (4608 x 2048: 12.1 against 16.1): left to a rule of its own.
 struct MmPlan {
   int tile;
   long long units;

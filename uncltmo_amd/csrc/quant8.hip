@@ -4,9 +4,10 @@
 //   scale = max(amax, 2^-100) fl(1 / top),   q = round_even(x fl(1 / scale))
 //
 // One pass: a block is read once, its maximum found in registers (and LDS), and written in 8 bits: bound by HBM, 2 (or 4) + 1 bytes an
-// element.  Both ways from one read (1 + 1 bytes written): 4099 x 2048 bf16 15.5 us = 2.2 TB/s, with the columns' sums 4099 x 4096 24.6 us
-// = 2.7 TB/s -- 528 and 1056 workgroups of one tile each, two to a CU, whose read, maxima, conversion and writes follow one another: the
-// short grids leave little of another tile's traffic to fill the gaps.
+// element.  By rows, bf16: 28800 x 256 7.4 us = 3.0 TB/s, 8192 x 4096 20.3 us = 5.0 TB/s.  Tiles: 4099 x 2048 8.6 us = 2.9 TB/s; transposed rows
+// 10.6 us, transposed tiles of 4099 x 4096 14.0 us = 3.6 TB/s.  Both ways from one read (1 + 1 bytes written): 4099 x 2048 15.5 us = 2.2 TB/s, with
+// the columns' sums 4099 x 4096 24.8 us = 2.7 TB/s -- 528 and 1056 workgroups of one tile each, whose read, maxima, conversion and writes
+// follow one another at the same time on every CU: the short grids leave little of another tile's traffic to fill the gaps.
 #include "matmul8_args.h"
 #include "row_ops.h"
 
@@ -46,7 +47,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const QuantArgs a) {
 // One workgroup, one 128 x 128 tile of x, an 8 x 8 patch a thread, read once.  TILE: one scale for the tile, else one for each row's 128
 // (q) and one for each column's 128 (its transpose).  WAYS: 1 = q as x lies, 2 = transposed, 3 = both; SUMS: the columns' sums too (the bias
 // gradient of a linear layer whose output gradient this is), as partial sums [tiles of rows][cols].  The bytes of the transpose turn
-// round in LDS: rows of 132 bytes put the eight lanes that write at once eight banks apart.
+// round in LDS: rows of 132 bytes put the eight lanes that write at once eight banks apart (384 cycles of conflicts are left in a workgroup).
 // eight neighbours of a row as they lie in memory; their sizes (bits without the sign) compare as integers of the type's own width, two at a
 // time for the 16-bit types
 template <typename T>

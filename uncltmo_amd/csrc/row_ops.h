@@ -66,7 +66,8 @@ struct RoRaw8 {
 };
 
 // up to eight elements of each of two rows (q NULL: of one, and b is 0); both loads go out before either is waited for where all eight exist
-// (the norm's backward pass of 508032 x 32 bf16 25.2 -> 21.4 us with gh's load as early; dropout, whose flags the first wait hides, lost 8 %)
+// (bf16, inputs of four sets in turn: the norm of 508032 x 32 28.4 -> 26.2 us, its backward pass, with gh's load as early, 28.8 -> 27.5 and of
+// 20000 x 4096 133 -> 120; dropout, whose flags the first wait hides, lost 8 %)
 template <typename T>
 __device__ __forceinline__ void ro_load8_two(const T* p, const T* q, int n, float* a, float* b) {
   if (n >= 8) {

@@ -11,8 +11,8 @@
 // into a wave, so that every access of a wave is 1 KB of consecutive memory whatever the width.
 //
 // Measured, bf16 (a copy of 1 GiB runs at 5.05 TB/s on the same card): dropout of 16 x 252 x 252 x 32 25.6 us = 5.1 TB/s (a Philox
-// evaluation of ten rounds for each eight elements hides behind the loads); addition and norm of 8 x 252 x 252 x 32 28.4 us = 4.6 TB/s,
-// the backward pass 24.9 us = 5.2 TB/s and 4.1 us for the weight gradient's fold; into 8 bits 28800 x 256 11.5 us = 4.6 TB/s; a single row
+// evaluation of ten rounds for each eight elements hides behind the loads); addition and norm of 8 x 252 x 252 x 32 28.3 us = 4.6 TB/s,
+// the backward pass 25.4 us = 5.1 TB/s and 4.0 us for the weight gradient's fold; into 8 bits 28800 x 256 11.9 us = 4.4 TB/s; a single row
 // 3.4 us, of which the launch is most.
 #include "row_ops.h"
 
