@@ -3,8 +3,10 @@ not come back in an A/B or timing build, and objects compiled with other flags a
 import glob
 import os
 import re
+import types
 
 import __graft_entry__ as ge
+from uncltmo_amd import _hip
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -39,6 +41,8 @@ def test_objects_compiled_with_other_flags_are_not_kept(monkeypatch, tmp_path):
 
         def wait(self):
             return 0
+    monkeypatch.setattr(_hip, "lib", lambda: types.SimpleNamespace(uncl_version=lambda: 1))
+    monkeypatch.syspath_prepend(str(tmp_path))
     monkeypatch.setattr(ge, "ROOT", str(tmp_path))
     monkeypatch.setattr(ge, "CSRC", str(csrc))
     monkeypatch.setattr(ge, "LIB", str(tmp_path / "lib.so"))
